@@ -33,6 +33,7 @@ extern "C" {
 #define QGEMM_DT_F16 0
 #define QGEMM_DT_BF16 1
 #define QGEMM_DT_I32 2
+#define QGEMM_DT_F32 3
 
 #define QGEMM_B_KN 0 /* B stored [batch, K, N], N contiguous (examples/quant_batch_matmul) */
 #define QGEMM_B_NK 1 /* B stored [batch, N, K], K contiguous (examples/deepseek_v4/int8_gemm.py:58) */
@@ -335,6 +336,74 @@ int qgemm_w4a8_act_quant(const void* X, int x_dtype, const uint8_t* qB, int8_t* 
  */
 int qgemm_act_quant(const void* X, int8_t* Y, float* S, int64_t M, int64_t N, int x_dtype, int round_scale,
                     void* stream);
+
+/*
+ * What a mixture layer runs around the grouped product: qgemm_moe_route -> qgemm_moe_blocks -> qgemm_moe_act_quant ->
+ * qgemm_w8a8_grouped_zeroed -> qgemm_swiglu_act_quant -> qgemm_w8a8_grouped_zeroed -> qgemm_moe_combine.  Nothing of it
+ * is read back by the host, so that the whole layer can be captured in a graph.  (No counterparts in the reference,
+ * whose grouped GEMM starts from sorted rows and a host-built table, example_grouped_gemm_fwd.py:147-166.)
+ *
+ * Routing.  For every token, with l its logits and s = softmax(l) or sigmoid(l):
+ *   c[e]       = s[e] (+ bias[e]);  expert e is offered if l[e] > -inf and c[e] > -inf
+ *   groups     = num_groups runs of E / num_groups experts; a group is worth the sum of its group_top (1 or 2) largest
+ *                offered c; the top_groups most valuable ones stay (ties: the lower index)
+ *   experts    = the top_k largest c offered in groups that stay, in that order (ties: the lower index), -1 where
+ *                there are no more
+ *   weights[j] = s[experts[j]], with `renormalize` divided by their sum, times `scale`; 0 where there is no expert
+ * The picks are those of the exact scores (without a bias the logits are compared; with one, decisions that are nearer
+ * than the error of fp32 are taken in fp64).  A NaN counts as largest and makes its weights NaN.
+ * logits: [T, E] F16 / BF16 / F32.  bias: nullable fp32 [E].  weights: [T, top_k] fp32.  experts: [T, top_k] int32.
+ * E <= 1024, top_k <= 32, num_groups <= 32.
+ */
+#define QGEMM_ROUTE_SOFTMAX 0
+#define QGEMM_ROUTE_SIGMOID 1
+int qgemm_moe_route(const void* logits, const float* bias, float* weights, int32_t* experts, int64_t T, int64_t E,
+                    int64_t top_k, int64_t num_groups, int64_t top_groups, int group_top, int scoring, int renormalize,
+                    float scale, int logits_dtype, void* stream);
+
+/*
+ * Tables of the grouped product from routed experts, on the device.  `experts` holds `entries` picks (tokens x top_k); one
+ * outside 0 .. num_experts - 1 is dropped.  The picks are stacked expert by expert, in their own order within one,
+ * the dropped ones behind all others:
+ *   sizes[e]       = picks of expert e                                                        int32 [num_experts]
+ *   rows[i]        = place of pick i in the stack, or -2 - place if it is dropped             int32 [entries]
+ *   block_metadata = (expert, first row, valid rows) of every block of up to block_M rows     int32 [blocks, 3]
+ * as construct_inputs builds the table (example_grouped_gemm_fwd.py:147-166).  blocks = qgemm_moe_block_count(): what
+ * the picks can need at most; entries without a block are (-1, entries, 0), which qgemm_w8a8_grouped skips.
+ * num_experts <= 1024, block_M <= 128.
+ */
+int64_t qgemm_moe_block_count(int64_t entries, int64_t num_experts, int64_t block_M);
+int qgemm_moe_blocks(const int32_t* experts, int32_t* block_metadata, int32_t* rows, int32_t* sizes, int64_t entries,
+                     int64_t num_experts, int64_t block_M, void* stream);
+
+/*
+ * qgemm_act_quant of X [T, N] with every row and its scale written to the token's top_k places rows[t, :] of Y [T * top_k, N] and
+ * S [T * top_k]: the grouped product's A and scale_a.  Same arithmetic, bit for bit.  A place -2 - r (dropped by
+ * qgemm_moe_blocks) clears row r of Y and S; any other place outside Y is passed over.  No two entries may
+ * name the same row.  X 16-byte, Y 8-byte aligned, N % 8 == 0.
+ */
+int qgemm_moe_act_quant(const void* X, const int32_t* rows, int8_t* Y, float* S, int64_t T, int64_t N, int64_t top_k,
+                        int x_dtype, int round_scale, void* stream);
+
+/*
+ * Gated activation and quantiser between the experts' two products.  X: [M, 2 F] F16 / BF16, gate columns first.
+ *   a[m, f] = silu(X[m, f]) * X[m, F + f]        silu(g) = g / (1 + exp(-g))
+ *   S[m]    = max(max_f |a[m, f]|, 1e-4) / 127   rounded to fp32 (round_scale != 0: then up to a power of two)
+ *   Y[m, f] = int8( a[m, f] / S[m] to the nearest integer )
+ * with a and the quotient exact: where fp32 cannot tell which integer is nearer, fp64 decides.  In a row with an infinity or a NaN
+ * S is one and Y unspecified.  X 16-byte, Y 8-byte aligned, F % 8 == 0.
+ */
+int qgemm_swiglu_act_quant(const void* X, int8_t* Y, float* S, int64_t M, int64_t F, int x_dtype, int round_scale,
+                           void* stream);
+
+/*
+ * The experts' outputs back in the tokens' order:
+ *   out[t, :] = cast( (base[t, :]) + sum_j weights[t, j] * Y[rows[t, j], :] )        fp32, j ascending, one rounding at the end
+ * Y: [R, N], base (nullable) and out: [T, N], all of `dtype` (F16 / BF16).  An entry of `rows` outside 0 .. R - 1 adds
+ * nothing, whatever its weight.  out may be base.  All 16-byte aligned, N % 8 == 0.
+ */
+int qgemm_moe_combine(const void* Y, const int32_t* rows, const float* weights, const void* base, void* out, int64_t R,
+                      int64_t T, int64_t N, int64_t top_k, int dtype, void* stream);
 
 #ifdef __cplusplus
 }

@@ -21,6 +21,13 @@ from .ops import (  # noqa: F401
     w4a8_gemm_cv,
     w4a8_gemm_act_quant,
 )
+from .moe import (  # noqa: F401
+    moe_act_quant,
+    moe_block_metadata,
+    moe_combine,
+    moe_route,
+    swiglu_act_quant,
+)
 from .quantize import (  # noqa: F401
     deinterleave_weight_int4_f16,
     gen_quant4,

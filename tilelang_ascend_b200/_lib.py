@@ -17,7 +17,7 @@ import warnings
 PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("QGEMM_LIB") or os.path.join(PKG, "libqgemm.so")  # QGEMM_LIB: another build of the library
 
-DT_F16, DT_BF16, DT_I32 = 0, 1, 2
+DT_F16, DT_BF16, DT_I32, DT_F32 = 0, 1, 2, 3
 B_KN, B_NK = 0, 1
 
 STATUS_NAMES = {0: "ok", 1: "timeout in TMA producer", 2: "timeout in MMA issuer", 3: "timeout in epilogue",
@@ -74,6 +74,17 @@ SIGNATURES = {
                                         _c.c_int64, _c.c_int64, _c.c_int64, _c.c_int, _c.c_void_p, _c.c_void_p]),
     "qgemm_act_quant": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_int, _c.c_int,
                                    _c.c_void_p]),
+    "qgemm_moe_route": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_int64,
+                                   _c.c_int64, _c.c_int64, _c.c_int, _c.c_int, _c.c_int, _c.c_float, _c.c_int, _c.c_void_p]),
+    "qgemm_moe_block_count": (_c.c_int64, [_c.c_int64, _c.c_int64, _c.c_int64]),
+    "qgemm_moe_blocks": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_int64,
+                                    _c.c_void_p]),
+    "qgemm_moe_act_quant": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_int64,
+                                       _c.c_int, _c.c_int, _c.c_void_p]),
+    "qgemm_swiglu_act_quant": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int64, _c.c_int, _c.c_int,
+                                          _c.c_void_p]),
+    "qgemm_moe_combine": (_c.c_int, [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int64,
+                                     _c.c_int64, _c.c_int64, _c.c_int, _c.c_void_p]),
 }
 
 _lock = threading.RLock()

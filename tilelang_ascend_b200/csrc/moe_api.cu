@@ -1,0 +1,232 @@
+// Host side of the operators around the experts' products (qgemm_moe_*, qgemm_swiglu_act_quant): argument validation, choice
+// of launch shapes.  The exported functions are declared and documented in include/qgemm.h.
+#include "../../include/qgemm.h"
+
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+#include "host_common.cuh"
+#include "moe_blocks.cuh"
+#include "moe_route.cuh"
+#include "moe_rows.cuh"
+#include "swiglu_quant.cuh"
+
+namespace {
+
+using namespace qgh;
+
+bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+template <int DT>
+int launch_route(const qg::MoeRouteParams& p, int sms, cudaStream_t s) {
+  const long long blocks = std::min<long long>((p.T + qg::RT_WARPS - 1) / qg::RT_WARPS, 16ll * sms);
+  const int smem = qg::RT_WARPS * 8 * p.E;
+  auto launch = [&](auto kernel) { return launch_pdl(kernel, (int)blocks, qg::RT_WARPS * 32, smem, s, p); };
+  if (p.E <= 32) return launch(qg::moe_route_kernel<DT, 1>);
+  if (p.E <= 64) return launch(qg::moe_route_kernel<DT, 2>);
+  if (p.E <= 128) return launch(qg::moe_route_kernel<DT, 4>);
+  if (p.E <= 256) return launch(qg::moe_route_kernel<DT, 8>);
+  if (p.E <= 512) return launch(qg::moe_route_kernel<DT, 16>);
+  return launch(qg::moe_route_kernel<DT, 32>);
+}
+
+// Once per device: the block-table kernel's shared memory and its clusters of more than eight CTAs.
+constexpr int kMaxDevices = 64;
+int ensure_blocks_kernel() {
+  static std::atomic<bool> ready[kMaxDevices];
+  int dev = 0;
+  CUDA_OK(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= kMaxDevices) return fail("device index %d out of range", dev);
+  if (ready[dev].load(std::memory_order_acquire)) return 0;
+  CUDA_OK(cudaFuncSetAttribute(qg::moe_blocks_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               qg::mb_smem_bytes(qg::MB_MAX_THREADS, qg::MB_MAX_E)));
+  CUDA_OK(cudaFuncSetAttribute(qg::moe_blocks_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+  ready[dev].store(true, std::memory_order_release);
+  return 0;
+}
+
+}  // namespace
+
+extern "C" {
+
+int qgemm_moe_route(const void* logits, const float* bias, float* weights, int32_t* experts, int64_t T, int64_t E, int64_t top_k,
+                    int64_t num_groups, int64_t top_groups, int group_top, int scoring, int renormalize, float scale, int logits_dtype,
+                    void* stream) {
+  if (T < 0 || T > (1ll << 30)) return fail("qgemm_moe_route: 0 to 2^30 tokens (got %lld)", (long long)T);
+  if (E < 1 || E > qg::RT_MAX_E) return fail("qgemm_moe_route: 1 to %d experts (got %lld)", qg::RT_MAX_E, (long long)E);
+  if (num_groups < 1 || num_groups > qg::RT_MAX_GROUPS || E % num_groups != 0)
+    return fail("qgemm_moe_route: num_groups must be 1 to %d and divide the number of experts (got %lld groups, %lld experts)",
+                qg::RT_MAX_GROUPS, (long long)num_groups, (long long)E);
+  if (top_groups < 1 || top_groups > num_groups)
+    return fail("qgemm_moe_route: top_groups must be 1 to num_groups (got %lld of %lld)", (long long)top_groups, (long long)num_groups);
+  if (top_k < 1 || top_k > qg::RT_MAX_K || top_k > E / num_groups * top_groups)
+    return fail("qgemm_moe_route: top_k must be 1 to %d and no more than the %lld experts of top_groups groups (got %lld)", qg::RT_MAX_K,
+                (long long)(E / num_groups * top_groups), (long long)top_k);
+  if (group_top != 1 && group_top != 2) return fail("qgemm_moe_route: group_top must be 1 or 2 (got %d)", group_top);
+  if (scoring != QGEMM_ROUTE_SOFTMAX && scoring != QGEMM_ROUTE_SIGMOID) return fail("qgemm_moe_route: unknown scoring %d", scoring);
+  if (logits_dtype != QGEMM_DT_F16 && logits_dtype != QGEMM_DT_BF16 && logits_dtype != QGEMM_DT_F32)
+    return fail("qgemm_moe_route: logits_dtype must be F16, BF16 or F32 (got %d)", logits_dtype);
+  if (T == 0) return 0;
+  if (logits == nullptr || weights == nullptr || experts == nullptr) return fail("qgemm_moe_route: null pointer");
+  if (!aligned(logits, logits_dtype == QGEMM_DT_F32 ? 4 : 2) || !aligned(bias, 4) || !aligned(weights, 4) || !aligned(experts, 4))
+    return fail("qgemm_moe_route: pointers must be aligned to their elements");
+  int sms = 0;
+  if (ensure_device(&sms)) return -1;
+  qg::MoeRouteParams p;
+  p.logits = logits;
+  p.bias = bias;
+  p.weights = weights;
+  p.experts = experts;
+  p.T = T;
+  p.E = (int)E;
+  p.k = (int)top_k;
+  p.groups = top_groups == num_groups ? 1 : (int)num_groups;  // all groups stay: nothing to choose
+  p.group_n = (int)(E / p.groups);
+  p.top_groups = p.groups == 1 ? 1 : (int)top_groups;
+  p.group_top = group_top;
+  p.softmax = scoring == QGEMM_ROUTE_SOFTMAX;
+  p.renormalize = renormalize != 0;
+  p.scale = scale;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (logits_dtype == QGEMM_DT_F32) return launch_route<qg::RT_F32>(p, sms, s);
+  return logits_dtype == QGEMM_DT_BF16 ? launch_route<qg::RT_BF16>(p, sms, s) : launch_route<qg::RT_F16>(p, sms, s);
+}
+
+int64_t qgemm_moe_block_count(int64_t entries, int64_t num_experts, int64_t block_M) {
+  if (entries <= 0 || num_experts <= 0 || block_M <= 0) return 0;
+  const int64_t n = std::min(entries, num_experts);
+  return n + (entries - n) / block_M;
+}
+
+int qgemm_moe_blocks(const int32_t* experts, int32_t* block_metadata, int32_t* rows, int32_t* sizes, int64_t entries, int64_t num_experts,
+                     int64_t block_M, void* stream) {
+  if (entries < 0 || entries > (1ll << 30)) return fail("qgemm_moe_blocks: 0 to 2^30 entries (got %lld)", (long long)entries);
+  if (num_experts < 1 || num_experts > qg::MB_MAX_E) return fail("qgemm_moe_blocks: 1 to %d experts (got %lld)", qg::MB_MAX_E, (long long)num_experts);
+  if (block_M < 1 || block_M > 128) return fail("qgemm_moe_blocks: block_M must be 1 to 128 (got %lld)", (long long)block_M);
+  if (sizes == nullptr || (entries > 0 && (experts == nullptr || block_metadata == nullptr || rows == nullptr)))
+    return fail("qgemm_moe_blocks: null pointer");
+  if (!aligned(experts, 4) || !aligned(block_metadata, 4) || !aligned(rows, 4) || !aligned(sizes, 4))
+    return fail("qgemm_moe_blocks: pointers must be 4-byte aligned");
+  int sms = 0;
+  if (ensure_device(&sms) || ensure_blocks_kernel()) return -1;
+  qg::MoeBlocksParams p;
+  p.experts = experts;
+  p.meta = block_metadata;
+  p.rows = rows;
+  p.sizes = sizes;
+  p.R = (int)entries;
+  p.E = (int)num_experts;
+  p.block_m = (int)block_M;
+  p.blocks = (int)qgemm_moe_block_count(entries, num_experts, block_M);
+  const int threads = entries <= 2048 ? 256 : qg::MB_MAX_THREADS;
+  int ctas = 1;
+  while (ctas < qg::MB_MAX_CLUSTER && entries > 4096ll * ctas) ctas *= 2;
+  return launch_pdl_clusters(qg::moe_blocks_kernel, ctas, ctas, threads, qg::mb_smem_bytes(threads, p.E), static_cast<cudaStream_t>(stream), p);
+}
+
+int qgemm_moe_act_quant(const void* X, const int32_t* rows, int8_t* Y, float* S, int64_t T, int64_t N, int64_t top_k, int x_dtype,
+                        int round_scale, void* stream) {
+  if (T < 0 || N <= 0 || (N % 8) != 0)
+    return fail("qgemm_moe_act_quant: T >= 0 and N a positive multiple of 8 required (got T=%lld, N=%lld)", (long long)T, (long long)N);
+  if (N > (1ll << 30)) return fail("qgemm_moe_act_quant: N too large (%lld)", (long long)N);
+  if (top_k < 1 || T > (1ll << 30) || T * top_k > (1ll << 30))
+    return fail("qgemm_moe_act_quant: top_k >= 1 and no more than 2^30 rows required (got T=%lld, top_k=%lld)", (long long)T, (long long)top_k);
+  if (x_dtype != QGEMM_DT_F16 && x_dtype != QGEMM_DT_BF16) return fail("qgemm_moe_act_quant: x_dtype must be F16 or BF16 (got %d)", x_dtype);
+  if (T == 0) return 0;
+  if (X == nullptr || rows == nullptr || Y == nullptr || S == nullptr) return fail("qgemm_moe_act_quant: null pointer");
+  if (!aligned16(X) || !aligned(Y, 8) || !aligned(S, 4) || !aligned(rows, 4))
+    return fail("qgemm_moe_act_quant: X must be 16-byte, Y 8-byte, S and rows 4-byte aligned");
+  int sms = 0;
+  if (ensure_device(&sms)) return -1;
+  qg::MoeActQuantParams p;
+  p.X = static_cast<const uint4*>(X);
+  p.rows = rows;
+  p.Y = Y;
+  p.S = S;
+  p.T = T;
+  p.N = (int)N;
+  p.k = (int)top_k;
+  p.is_bf16 = x_dtype == QGEMM_DT_BF16;
+  p.round_scale = round_scale != 0;
+  const int64_t chunks = N / 8;
+  int tpr = 32;
+  while (tpr < 256 && chunks > (int64_t)tpr * 4) tpr *= 2;
+  const int64_t rows_per_block = qg::aq_block(tpr) / tpr, grid = (T + rows_per_block - 1) / rows_per_block;
+  auto launch = [&](auto kernel) { return launch_pdl(kernel, (int)grid, qg::aq_block(tpr), 0, static_cast<cudaStream_t>(stream), p); };
+  if (tpr == 32) return launch(qg::moe_act_quant_kernel<32, 4>);
+  if (tpr == 64) return launch(qg::moe_act_quant_kernel<64, 4>);
+  if (tpr == 128) return launch(qg::moe_act_quant_kernel<128, 4>);
+  return launch(qg::moe_act_quant_kernel<256, 4>);
+}
+
+int qgemm_swiglu_act_quant(const void* X, int8_t* Y, float* S, int64_t M, int64_t F, int x_dtype, int round_scale, void* stream) {
+  if (M < 0 || F <= 0 || (F % 8) != 0)
+    return fail("qgemm_swiglu_act_quant: M >= 0 and F a positive multiple of 8 required (got M=%lld, F=%lld)", (long long)M, (long long)F);
+  if (F > (1ll << 29)) return fail("qgemm_swiglu_act_quant: F too large (%lld)", (long long)F);
+  if (x_dtype != QGEMM_DT_F16 && x_dtype != QGEMM_DT_BF16) return fail("qgemm_swiglu_act_quant: x_dtype must be F16 or BF16 (got %d)", x_dtype);
+  if (M == 0) return 0;
+  if (X == nullptr || Y == nullptr || S == nullptr) return fail("qgemm_swiglu_act_quant: null pointer");
+  if (!aligned16(X) || !aligned(Y, 8) || !aligned(S, 4))
+    return fail("qgemm_swiglu_act_quant: X must be 16-byte, Y 8-byte and S 4-byte aligned");
+  int sms = 0;
+  if (ensure_device(&sms)) return -1;
+  qg::SwigluQuantParams p;
+  p.X = static_cast<const uint4*>(X);
+  p.Y = Y;
+  p.S = S;
+  p.M = M;
+  p.F = (int)F;
+  p.round_scale = round_scale != 0;
+  const int64_t chunks = F / 8;
+  int tpr = 32;
+  while (tpr < 256 && chunks > tpr) tpr *= 2;
+  const int64_t rows_per_block = qg::aq_block(tpr) / tpr, grid = (M + rows_per_block - 1) / rows_per_block;
+  if (grid > 0x7fffffffll) return fail("qgemm_swiglu_act_quant: too many rows (%lld)", (long long)M);
+  auto launch = [&](auto kernel) { return launch_pdl(kernel, (int)grid, qg::aq_block(tpr), 0, static_cast<cudaStream_t>(stream), p); };
+  auto launch_type = [&](auto bf16) {
+    constexpr bool BF16 = decltype(bf16)::value;
+    if (tpr == 32) return launch(qg::swiglu_quant_kernel<32, 1, BF16>);
+    if (tpr == 64) return launch(qg::swiglu_quant_kernel<64, 1, BF16>);
+    if (tpr == 128) return launch(qg::swiglu_quant_kernel<128, 1, BF16>);
+    if (chunks <= 256) return launch(qg::swiglu_quant_kernel<256, 1, BF16>);
+    if (chunks <= 512) return launch(qg::swiglu_quant_kernel<256, 2, BF16>);
+    return launch(qg::swiglu_quant_kernel<256, 4, BF16>);
+  };
+  return x_dtype == QGEMM_DT_BF16 ? launch_type(std::true_type{}) : launch_type(std::false_type{});
+}
+
+int qgemm_moe_combine(const void* Y, const int32_t* rows, const float* weights, const void* base, void* out, int64_t R, int64_t T, int64_t N,
+                      int64_t top_k, int dtype, void* stream) {
+  if (T < 0 || R < 0 || N <= 0 || (N % 8) != 0)
+    return fail("qgemm_moe_combine: T, R >= 0 and N a positive multiple of 8 required (got T=%lld, R=%lld, N=%lld)", (long long)T, (long long)R,
+                (long long)N);
+  if (N > (1ll << 30) || R > (1ll << 31)) return fail("qgemm_moe_combine: dimension too large (R=%lld, N=%lld)", (long long)R, (long long)N);
+  if (top_k < 1 || T > (1ll << 30) || T * top_k > (1ll << 30))
+    return fail("qgemm_moe_combine: top_k >= 1 and no more than 2^30 entries required (got T=%lld, top_k=%lld)", (long long)T, (long long)top_k);
+  if (dtype != QGEMM_DT_F16 && dtype != QGEMM_DT_BF16) return fail("qgemm_moe_combine: dtype must be F16 or BF16 (got %d)", dtype);
+  if (T == 0) return 0;
+  if ((Y == nullptr && R > 0) || rows == nullptr || weights == nullptr || out == nullptr) return fail("qgemm_moe_combine: null pointer");
+  if (!aligned16(Y) || !aligned16(base) || !aligned16(out) || !aligned(rows, 4) || !aligned(weights, 4))
+    return fail("qgemm_moe_combine: Y, base and out must be 16-byte, rows and weights 4-byte aligned");
+  int sms = 0;
+  if (ensure_device(&sms)) return -1;
+  qg::MoeCombineParams p;
+  p.Y = static_cast<const uint4*>(Y);
+  p.rows = rows;
+  p.weights = weights;
+  p.base = static_cast<const uint4*>(base);
+  p.out = static_cast<uint4*>(out);
+  p.R = R;
+  p.T = T;
+  p.N = (int)N;
+  p.k = (int)top_k;
+  p.parts = (int)((N / 8 + qg::MC_THREADS - 1) / qg::MC_THREADS);
+  const int64_t grid = T * p.parts;
+  if (grid > 0x7fffffffll) return fail("qgemm_moe_combine: too many tokens (%lld of %lld)", (long long)T, (long long)N);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return dtype == QGEMM_DT_BF16 ? launch_pdl(qg::moe_combine_kernel<true>, (int)grid, qg::MC_THREADS, 0, s, p)
+                                : launch_pdl(qg::moe_combine_kernel<false>, (int)grid, qg::MC_THREADS, 0, s, p);
+}
+
+}  // extern "C"

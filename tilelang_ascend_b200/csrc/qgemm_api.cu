@@ -10,6 +10,7 @@
 #include <cstring>
 #include <mutex>
 
+#include "host_common.cuh"
 #include "w4a16.cuh"
 #include "w4a16_decode.cuh"
 #include "w4a16_gs.cuh"
@@ -19,10 +20,9 @@
 #include "w8a8.cuh"
 #include "w8a8_rows.cuh"
 
-namespace {
+namespace qgh {
 
-thread_local char g_err[512] = "";
-unsigned long long g_wait_limit_ns = 2000ull * 1000ull * 1000ull;
+static thread_local char g_err[512] = "";
 
 int fail(const char* fmt, ...) {
   va_list ap;
@@ -32,11 +32,13 @@ int fail(const char* fmt, ...) {
   return -1;
 }
 
-#define CUDA_OK(expr)                                                                      \
-  do {                                                                                     \
-    cudaError_t e_ = (expr);                                                               \
-    if (e_ != cudaSuccess) return fail("%s failed: %s", #expr, cudaGetErrorString(e_));   \
-  } while (0)
+}  // namespace qgh
+
+namespace {
+
+using namespace qgh;
+
+unsigned long long g_wait_limit_ns = 2000ull * 1000ull * 1000ull;
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -144,8 +146,10 @@ int set_smem_w4w() {
   return set_smem(qg::w4a16_wide_kernel<true, true, PAIR>, qg::W4WideCfg<true>::SMEM_BYTES);
 }
 
+}  // namespace
+
 // The set-up of the current device, once per device.
-int ensure_device(int* sm_count) {
+int qgh::ensure_device(int* sm_count) {
   int dev = 0;
   CUDA_OK(cudaGetDevice(&dev));
   if (dev < 0 || dev >= kMaxDevices) return fail("device index %d out of range", dev);
@@ -182,6 +186,8 @@ int ensure_device(int* sm_count) {
   return 0;
 }
 
+namespace {
+
 // rank-2/3 row-major tensor map; dims/box innermost first; strides in bytes for dims 1.. (innermost is dense).
 int encode_map(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void* base, const uint64_t* dims,
                const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swz) {
@@ -197,28 +203,6 @@ int encode_map(CUtensorMap* map, CUtensorMapDataType dt, int rank, const void* b
                         CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return fail("cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
-  return 0;
-}
-
-bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-// Launch `kernel` so that it may start while the kernel in front of it on the stream is still running
-// (programmatic dependent launch); the kernel itself waits before it reads that kernel's results.
-// QGEMM_PDL=0 falls back to plain stream order.
-template <typename... KArgs, typename... Args>
-int launch_pdl(void (*kernel)(KArgs...), int grid, int threads, int smem, cudaStream_t s, Args&&... args) {
-  static const int pdl = getenv("QGEMM_PDL") ? atoi(getenv("QGEMM_PDL")) : 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = (size_t)smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl ? 1 : 0;
-  CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...));
   return 0;
 }
 
