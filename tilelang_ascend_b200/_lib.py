@@ -93,7 +93,8 @@ _host = None
 
 # entry points the native call path (csrc/host.cpp) is handed, in the order its init() takes them
 _HOST_ENTRY_POINTS = ("qgemm_w8a8", "qgemm_w8a8_grouped", "qgemm_w4a16_call_workspace_bytes", "qgemm_w4a16_ex", "qgemm_w4a8",
-                      "qgemm_w4a8_act_quant", "qgemm_act_quant", "qgemm_w8a8_grouped_zeroed")
+                      "qgemm_w4a8_act_quant", "qgemm_act_quant", "qgemm_w8a8_grouped_zeroed", "qgemm_moe_route",
+                      "qgemm_moe_block_count", "qgemm_moe_blocks", "qgemm_moe_act_quant", "qgemm_swiglu_act_quant", "qgemm_moe_combine")
 
 
 class QGemmError(RuntimeError):

@@ -35,6 +35,12 @@ struct Api {
   decltype(&qgemm_w4a8) w4a8 = nullptr;
   decltype(&qgemm_w4a8_act_quant) w4a8_aq = nullptr;
   decltype(&qgemm_act_quant) act_quant = nullptr;
+  decltype(&qgemm_moe_route) moe_route = nullptr;
+  decltype(&qgemm_moe_block_count) moe_block_count = nullptr;
+  decltype(&qgemm_moe_blocks) moe_blocks = nullptr;
+  decltype(&qgemm_moe_act_quant) moe_act_quant = nullptr;
+  decltype(&qgemm_swiglu_act_quant) swiglu_act_quant = nullptr;
+  decltype(&qgemm_moe_combine) moe_combine = nullptr;
 } api;
 
 using at::ScalarType;
@@ -101,9 +107,9 @@ struct WithoutGil {
   }
 
 PyObject* h_init(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  constexpr int kEntries = 8;
+  constexpr int kEntries = 14;
   if (n != kEntries) {
-    PyErr_SetString(PyExc_TypeError, "init takes the addresses of the eight entry points");
+    PyErr_SetString(PyExc_TypeError, "init takes the addresses of the fourteen entry points");
     return nullptr;
   }
   void* p[kEntries];
@@ -119,6 +125,12 @@ PyObject* h_init(PyObject*, PyObject* const* args, Py_ssize_t n) {
   api.w4a8_aq = reinterpret_cast<decltype(api.w4a8_aq)>(p[5]);
   api.act_quant = reinterpret_cast<decltype(api.act_quant)>(p[6]);
   api.w8a8_grouped_zeroed = reinterpret_cast<decltype(api.w8a8_grouped_zeroed)>(p[7]);
+  api.moe_route = reinterpret_cast<decltype(api.moe_route)>(p[8]);
+  api.moe_block_count = reinterpret_cast<decltype(api.moe_block_count)>(p[9]);
+  api.moe_blocks = reinterpret_cast<decltype(api.moe_blocks)>(p[10]);
+  api.moe_act_quant = reinterpret_cast<decltype(api.moe_act_quant)>(p[11]);
+  api.swiglu_act_quant = reinterpret_cast<decltype(api.swiglu_act_quant)>(p[12]);
+  api.moe_combine = reinterpret_cast<decltype(api.moe_combine)>(p[13]);
   Py_RETURN_NONE;
 }
 
@@ -173,6 +185,23 @@ PyObject* h_w8a8(PyObject*, PyObject* const* args, Py_ssize_t n) {
   QHOST_CATCH
 }
 
+// The tensors as a tuple of their Python objects; nullptr, with the error set, where that fails.
+template <typename... T>
+PyObject* wrap_all(T&&... tensors) {
+  PyObject* res = PyTuple_New(sizeof...(tensors));
+  if (res == nullptr) return nullptr;
+  Py_ssize_t i = 0;
+  auto put = [&](at::Tensor&& t) {
+    PyObject* o = THPVariable_Wrap(std::move(t));
+    if (o == nullptr) return false;
+    PyTuple_SET_ITEM(res, i++, o);
+    return true;
+  };
+  if ((put(std::move(tensors)) && ...)) return res;
+  Py_DECREF(res);
+  return nullptr;
+}
+
 // act_quant(x, round_scale) -> (y, s); want_n >= 0: x is [M, want_n] and s comes back as [M]
 PyObject* h_act_quant(PyObject*, PyObject* const* args, Py_ssize_t n) {
   QHOST_TRY
@@ -201,22 +230,7 @@ PyObject* h_act_quant(PyObject*, PyObject* const* args, Py_ssize_t n) {
                        N, dt, rs, st);
   }
   if (rc != 0) Py_RETURN_NONE;
-  PyObject* py = THPVariable_Wrap(std::move(y));
-  PyObject* ps = THPVariable_Wrap(std::move(s));
-  if (py == nullptr || ps == nullptr) {
-    Py_XDECREF(py);
-    Py_XDECREF(ps);
-    return nullptr;
-  }
-  PyObject* res = PyTuple_New(2);
-  if (res == nullptr) {
-    Py_DECREF(py);
-    Py_DECREF(ps);
-    return nullptr;
-  }
-  PyTuple_SET_ITEM(res, 0, py);
-  PyTuple_SET_ITEM(res, 1, ps);
-  return res;
+  return wrap_all(std::move(y), std::move(s));
   QHOST_CATCH
 }
 
@@ -403,10 +417,159 @@ PyObject* h_grouped(PyObject*, PyObject* const* args, Py_ssize_t n) {
   QHOST_CATCH
 }
 
+// A plain f16 / bf16 tensor.
+const at::Tensor* plain_half(PyObject* o) {
+  const at::Tensor* t = plain(o, at::kBFloat16);
+  return t != nullptr ? t : plain(o, at::kHalf);
+}
+
+// moe_route(logits, top_k, bias | None, scoring: int, num_groups, top_groups, group_top, renormalize: bool, scale) -> (weights, experts)
+PyObject* h_moe_route(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  QHOST_TRY
+  if (n != 9) Py_RETURN_NONE;
+  const at::Tensor* l = plain(args[0], at::kFloat);
+  if (l == nullptr) l = plain_half(args[0]);
+  if (l == nullptr || l->dim() != 2) Py_RETURN_NONE;
+  const int64_t T = l->size(0), E = l->size(1);
+  const at::Tensor* b = nullptr;
+  if (args[2] != Py_None) {
+    b = plain(args[2], at::kFloat);
+    if (b == nullptr || b->dim() != 1 || b->size(0) != E || !same_device(*l, b)) Py_RETURN_NONE;
+  }
+  const int64_t k = as_int(args[1]), scoring = as_int(args[3]), groups = as_int(args[4]), top_groups = as_int(args[5]), group_top = as_int(args[6]);
+  if (T == 0 || k <= 0 || k > E || scoring < 0 || groups <= 0 || top_groups <= 0 || group_top < 1 || group_top > 2) Py_RETURN_NONE;
+  if (args[7] != Py_True && args[7] != Py_False) Py_RETURN_NONE;
+  if (!PyFloat_CheckExact(args[8])) Py_RETURN_NONE;
+  const float scale = (float)PyFloat_AS_DOUBLE(args[8]);
+  const int dev = l->get_device();
+  c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
+  at::Tensor w = empty_cuda({T, k}, at::kFloat, dev), e = empty_cuda({T, k}, at::kInt, dev);
+  void* st = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
+  const int dt = l->scalar_type() == at::kFloat ? QGEMM_DT_F32 : abi_dt(l->scalar_type()), renorm = args[7] == Py_True ? 1 : 0;
+  int rc;
+  {
+    WithoutGil unlocked;
+    rc = api.moe_route(l->const_data_ptr(), b ? static_cast<const float*>(b->const_data_ptr()) : nullptr, static_cast<float*>(w.mutable_data_ptr()),
+                       static_cast<int32_t*>(e.mutable_data_ptr()), T, E, k, groups, top_groups, (int)group_top, (int)scoring, renorm, scale, dt, st);
+  }
+  if (rc != 0) Py_RETURN_NONE;
+  return wrap_all(std::move(w), std::move(e));
+  QHOST_CATCH
+}
+
+// moe_blocks(experts, num_experts, block_M) -> (block_metadata, rows, sizes)
+PyObject* h_moe_blocks(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  QHOST_TRY
+  if (n != 3) Py_RETURN_NONE;
+  const at::Tensor* x = plain(args[0], at::kInt);
+  if (x == nullptr || x->dim() != 2 || x->numel() == 0) Py_RETURN_NONE;
+  const int64_t E = as_int(args[1]), bm = as_int(args[2]), R = x->numel();
+  if (E <= 0 || bm <= 0) Py_RETURN_NONE;
+  const int dev = x->get_device();
+  c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
+  at::Tensor meta = empty_cuda({api.moe_block_count(R, E, bm), 3}, at::kInt, dev), rows = empty_cuda(x->sizes(), at::kInt, dev),
+             sizes = empty_cuda({E}, at::kInt, dev);
+  void* st = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
+  int rc;
+  {
+    WithoutGil unlocked;
+    rc = api.moe_blocks(static_cast<const int32_t*>(x->const_data_ptr()), static_cast<int32_t*>(meta.mutable_data_ptr()),
+                        static_cast<int32_t*>(rows.mutable_data_ptr()), static_cast<int32_t*>(sizes.mutable_data_ptr()), R, E, bm, st);
+  }
+  if (rc != 0) Py_RETURN_NONE;
+  return wrap_all(std::move(meta), std::move(rows), std::move(sizes));
+  QHOST_CATCH
+}
+
+// moe_act_quant(x, rows, round_scale: bool) -> (y, s)
+PyObject* h_moe_act_quant(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  QHOST_TRY
+  if (n != 3) Py_RETURN_NONE;
+  const at::Tensor* x = plain_half(args[0]);
+  const at::Tensor* rows = plain(args[1], at::kInt);
+  if (x == nullptr || rows == nullptr || x->dim() != 2 || rows->dim() != 2 || !same_device(*x, rows)) Py_RETURN_NONE;
+  if (args[2] != Py_True && args[2] != Py_False) Py_RETURN_NONE;
+  const int64_t T = x->size(0), N = x->size(1), k = rows->size(1);
+  if (rows->size(0) != T || T == 0 || N == 0 || k == 0) Py_RETURN_NONE;
+  const int dev = x->get_device();
+  c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
+  at::Tensor y = empty_cuda({T * k, N}, at::kChar, dev), s = empty_cuda({T * k, 1}, at::kFloat, dev);
+  void* st = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
+  const int dt = abi_dt(x->scalar_type()), rs = args[2] == Py_True ? 1 : 0;
+  int rc;
+  {
+    WithoutGil unlocked;
+    rc = api.moe_act_quant(x->const_data_ptr(), static_cast<const int32_t*>(rows->const_data_ptr()), static_cast<int8_t*>(y.mutable_data_ptr()),
+                           static_cast<float*>(s.mutable_data_ptr()), T, N, k, dt, rs, st);
+  }
+  if (rc != 0) Py_RETURN_NONE;
+  return wrap_all(std::move(y), std::move(s));
+  QHOST_CATCH
+}
+
+// swiglu_act_quant(x, round_scale: bool) -> (y, s)
+PyObject* h_swiglu_act_quant(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  QHOST_TRY
+  if (n != 2) Py_RETURN_NONE;
+  const at::Tensor* x = plain_half(args[0]);
+  if (x == nullptr || (args[1] != Py_True && args[1] != Py_False)) Py_RETURN_NONE;
+  const int64_t nd = x->dim();
+  if ((nd != 2 && nd != 3) || x->numel() == 0 || x->size(-1) % 2 != 0) Py_RETURN_NONE;
+  const int64_t F = x->size(-1) / 2, M = x->numel() / (2 * F);
+  const int dev = x->get_device();
+  c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
+  const int64_t ys[3] = {x->size(0), nd == 3 ? x->size(1) : F, F}, ss[3] = {x->size(0), nd == 3 ? x->size(1) : 1, 1};
+  at::Tensor y = empty_cuda(at::IntArrayRef(ys, (size_t)nd), at::kChar, dev), s = empty_cuda(at::IntArrayRef(ss, (size_t)nd), at::kFloat, dev);
+  void* st = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
+  const int dt = abi_dt(x->scalar_type()), rs = args[1] == Py_True ? 1 : 0;
+  int rc;
+  {
+    WithoutGil unlocked;
+    rc = api.swiglu_act_quant(x->const_data_ptr(), static_cast<int8_t*>(y.mutable_data_ptr()), static_cast<float*>(s.mutable_data_ptr()), M, F, dt,
+                              rs, st);
+  }
+  if (rc != 0) Py_RETURN_NONE;
+  return wrap_all(std::move(y), std::move(s));
+  QHOST_CATCH
+}
+
+// moe_combine(y, rows, weights, base | None) -> out
+PyObject* h_moe_combine(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  QHOST_TRY
+  if (n != 4) Py_RETURN_NONE;
+  const at::Tensor* y = plain_half(args[0]);
+  const at::Tensor* rows = plain(args[1], at::kInt);
+  const at::Tensor* w = plain(args[2], at::kFloat);
+  if (y == nullptr || rows == nullptr || w == nullptr || y->dim() != 2 || rows->dim() != 2 || w->dim() != 2) Py_RETURN_NONE;
+  const int64_t R = y->size(0), N = y->size(1), T = rows->size(0), k = rows->size(1);
+  if (w->size(0) != T || w->size(1) != k || !same_device(*y, rows) || !same_device(*y, w) || T * N * k == 0) Py_RETURN_NONE;
+  const at::Tensor* base = nullptr;
+  if (args[3] != Py_None) {
+    base = plain(args[3], y->scalar_type());
+    if (base == nullptr || base->dim() != 2 || base->size(0) != T || base->size(1) != N || !same_device(*y, base)) Py_RETURN_NONE;
+  }
+  const int dev = y->get_device();
+  c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
+  at::Tensor out = empty_cuda({T, N}, y->scalar_type(), dev);
+  void* st = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
+  const int dt = abi_dt(y->scalar_type());
+  int rc;
+  {
+    WithoutGil unlocked;
+    rc = api.moe_combine(y->const_data_ptr(), static_cast<const int32_t*>(rows->const_data_ptr()), static_cast<const float*>(w->const_data_ptr()),
+                         base ? base->const_data_ptr() : nullptr, out.mutable_data_ptr(), R, T, N, k, dt, st);
+  }
+  if (rc != 0) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(out));
+  QHOST_CATCH
+}
+
 #define QHOST_FN(name, fn) {name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(fn)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {QHOST_FN("init", h_init),       QHOST_FN("w8a8", h_w8a8),     QHOST_FN("act_quant", h_act_quant),
                          QHOST_FN("w4a16", h_w4a16),     QHOST_FN("w4a8", h_w4a8),     QHOST_FN("w4a8_aq", h_w4a8_aq),
-                         QHOST_FN("grouped", h_grouped), {nullptr, nullptr, 0, nullptr}};
+                         QHOST_FN("grouped", h_grouped), QHOST_FN("moe_route", h_moe_route), QHOST_FN("moe_blocks", h_moe_blocks),
+                         QHOST_FN("moe_act_quant", h_moe_act_quant), QHOST_FN("swiglu_act_quant", h_swiglu_act_quant),
+                         QHOST_FN("moe_combine", h_moe_combine), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_qhost", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -17,7 +17,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _lib
+from . import _lib, ops
 from .ops import _check_tensor, _ptr, _require_cuda, _stream_handle
 
 _ROUTE_DT = {torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16, torch.float32: _lib.DT_F32}
@@ -51,6 +51,10 @@ def moe_route(logits, top_k, bias=None, scoring="softmax", num_groups=1, top_gro
 
     An expert whose logit (or bias) is -inf is never chosen; where a token has fewer than ``top_k`` left, its last experts are
     -1 with weight 0 (a padding token: a row of -inf).  A NaN counts as largest and makes its token's weights NaN."""
+    if stream is None and scoring in _SCORING:
+        we = (ops._host or ops._native()).moe_route(logits, top_k, bias, _SCORING[scoring], num_groups, top_groups, group_top, renormalize, scale)
+        if we is not None:
+            return we
     lib = _lib.load()
     _check_2d(logits, 0, "logits", tuple(_ROUTE_DT))
     dev = logits.device
@@ -78,6 +82,10 @@ def moe_block_metadata(experts, num_experts, block_M=128, stream=None):
     ``(-1, T * top_k, 0)``, which the grouped product skips, up to the largest table that so many picks can need: the host
     does not learn the sizes.  A pick outside ``0 .. num_experts - 1`` (-1) is dropped: it takes a place behind all
     others, ``rows`` holds ``-2 - place``, and no block covers it."""
+    if stream is None:
+        tables = (ops._host or ops._native()).moe_blocks(experts, num_experts, block_M)
+        if tables is not None:
+            return tables
     lib = _lib.load()
     _check_2d(experts, 0, "experts", (torch.int32,))
     dev = experts.device
@@ -98,6 +106,10 @@ def moe_act_quant(x, rows, round_scale: bool = False, stream=None):
     Each token is quantised as by ``act_quant``, bit for bit, and written to its ``top_k`` places: ``A`` and ``scale_a`` of
     ``grouped_quant_matmul``.  The places of dropped picks are cleared.  ``rows`` names no place twice; a place that it names not
     at all is left as allocated."""
+    if stream is None:
+        ys = (ops._host or ops._native()).moe_act_quant(x, rows, round_scale)
+        if ys is not None:
+            return ys
     lib = _lib.load()
     _check_2d(x, 0, "x", tuple(_HALF_DT))
     dev = x.device
@@ -121,6 +133,10 @@ def swiglu_act_quant(x, round_scale: bool = False, stream=None):
     ``a = silu(gate) * up``; ``scale = max(max |a|, 1e-4) / 127`` in fp32 (a power of two not below it when ``round_scale``);
     ``y`` the integer nearest to ``a / scale``.  Both are those of the exact ``a``: no rounding of the product to 16 bits lies
     between, and values next to a border are decided in 64 bits."""
+    if stream is None:
+        ys = (ops._host or ops._native()).swiglu_act_quant(x, round_scale)
+        if ys is not None:
+            return ys
     lib = _lib.load()
     _require_cuda(x, "x")
     dev = x.device
@@ -148,6 +164,10 @@ def moe_combine(y, rows, weights, base=None, stream=None):
     ``rows`` [T, top_k] int32 as from ``moe_block_metadata`` (an entry outside ``0 .. R - 1`` adds nothing), ``weights`` [T, top_k] float32,
     ``base`` optional [T, N] of the type of ``y`` (a shared expert's output, a residual).  Summed in fp32, ``j`` ascending,
     rounded once."""
+    if stream is None:
+        out = (ops._host or ops._native()).moe_combine(y, rows, weights, base)
+        if out is not None:
+            return out
     lib = _lib.load()
     _check_2d(y, 0, "y", tuple(_HALF_DT))
     dev = y.device
