@@ -18,6 +18,27 @@ using namespace qgh;
 
 bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
+constexpr int kMaxDevices = 64;
+
+template <int TPR, int KEEP, bool BF16>
+int launch_swiglu(const qg::SwigluQuantParams& p, int sms, cudaStream_t s) {
+  auto kernel = qg::swiglu_quant_kernel<TPR, KEEP, BF16>;
+  constexpr int block = qg::sq_block(TPR), rows = block / TPR, smem = qg::sq_smem_bytes(TPR, KEEP);
+  static std::atomic<int> resident[kMaxDevices];  // blocks that an SM holds, once asked
+  int dev = 0, per_sm = 0;
+  CUDA_OK(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= kMaxDevices) return fail("device index %d out of range", dev);
+  if ((per_sm = resident[dev].load(std::memory_order_acquire)) == 0) {
+    CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+    CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, block, smem));
+    if (per_sm < 1) return fail("qgemm_swiglu_act_quant: the kernel does not fit on an SM");
+    resident[dev].store(per_sm, std::memory_order_release);
+  }
+  const int64_t grid = std::min<int64_t>((p.M + rows - 1) / rows, (int64_t)per_sm * sms);
+  return launch_pdl(kernel, (int)grid, block, smem, s, p);
+}
+
 template <int DT>
 int launch_route(const qg::MoeRouteParams& p, int sms, cudaStream_t s) {
   const long long blocks = std::min<long long>((p.T + qg::RT_WARPS - 1) / qg::RT_WARPS, 16ll * sms);
@@ -32,7 +53,6 @@ int launch_route(const qg::MoeRouteParams& p, int sms, cudaStream_t s) {
 }
 
 // Once per device: the block-table kernel's shared memory and its clusters of more than eight CTAs.
-constexpr int kMaxDevices = 64;
 int ensure_blocks_kernel() {
   static std::atomic<bool> ready[kMaxDevices];
   int dev = 0;
@@ -179,19 +199,52 @@ int qgemm_swiglu_act_quant(const void* X, int8_t* Y, float* S, int64_t M, int64_
   p.F = (int)F;
   p.round_scale = round_scale != 0;
   const int64_t chunks = F / 8;
-  int tpr = 32;
-  while (tpr < 256 && chunks > tpr) tpr *= 2;
-  const int64_t rows_per_block = qg::aq_block(tpr) / tpr, grid = (M + rows_per_block - 1) / rows_per_block;
-  if (grid > 0x7fffffffll) return fail("qgemm_swiglu_act_quant: too many rows (%lld)", (long long)M);
-  auto launch = [&](auto kernel) { return launch_pdl(kernel, (int)grid, qg::aq_block(tpr), 0, static_cast<cudaStream_t>(stream), p); };
-  auto launch_type = [&](auto bf16) {
+  // Threads per row and chunks of eight elements per thread.  While the rows leave threads idle, the fewest chunks that do not take more
+  // than 450 threads per SM; otherwise the shape with the fewest empty places, and of those the one with the fewest threads per row,
+  // whose maximum costs the least (a warp needs no barrier).  us, threads x chunks: 128 rows of 2048 256 x 1 2.5, 64 x 4 3.3, 32 x 8 4.0; 300 of
+  // 4096 256 x 2 4.05, 128 x 4 4.1, 64 x 8 4.6; 1200 of 768 64 x 2 3.8, 32 x 3 3.3; 1500 of 2048 32 x 8 5.9, 64 x 4 6.1; 32768 of 2048
+  // 32 x 8 63, 64 x 4 71; 8000 of 4096 64 x 8 34, 128 x 4 41; 5000 of 7168 128 x 7 41, 128 x 8 44, 256 x 4 52; 4000 of 14336 256 x 7 72,
+  // 512 x 4 88.
+  int keep = 0, tpr = 0;
+  for (int k = 1; k <= 4 && keep == 0; k *= 2) {
+    int t = 32;
+    while (t < 512 && chunks > (int64_t)t * k) t *= 2;
+    if (M * t <= 450ll * sms && chunks <= (int64_t)t * k) {
+      keep = (int)((chunks + t - 1) / t);
+      tpr = t;
+    }
+  }
+  if (keep == 0) {
+    keep = 8;
+    tpr = 512;
+    for (int t = 512; t >= 32; t /= 2) {
+      const int64_t k = (chunks + t - 1) / t;
+      if (k <= 8 && k * t <= (int64_t)keep * tpr) { keep = (int)k; tpr = t; }
+    }
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto launch_keep = [&](auto bf16, auto keep_) {
     constexpr bool BF16 = decltype(bf16)::value;
-    if (tpr == 32) return launch(qg::swiglu_quant_kernel<32, 1, BF16>);
-    if (tpr == 64) return launch(qg::swiglu_quant_kernel<64, 1, BF16>);
-    if (tpr == 128) return launch(qg::swiglu_quant_kernel<128, 1, BF16>);
-    if (chunks <= 256) return launch(qg::swiglu_quant_kernel<256, 1, BF16>);
-    if (chunks <= 512) return launch(qg::swiglu_quant_kernel<256, 2, BF16>);
-    return launch(qg::swiglu_quant_kernel<256, 4, BF16>);
+    constexpr int KEEP = decltype(keep_)::value;
+    switch (tpr) {
+      case 32: return launch_swiglu<32, KEEP, BF16>(p, sms, st);
+      case 64: return launch_swiglu<64, KEEP, BF16>(p, sms, st);
+      case 128: return launch_swiglu<128, KEEP, BF16>(p, sms, st);
+      case 256: return launch_swiglu<256, KEEP, BF16>(p, sms, st);
+      default: return launch_swiglu<512, KEEP, BF16>(p, sms, st);
+    }
+  };
+  auto launch_type = [&](auto bf16) {
+    switch (keep) {
+      case 1: return launch_keep(bf16, std::integral_constant<int, 1>{});
+      case 2: return launch_keep(bf16, std::integral_constant<int, 2>{});
+      case 3: return launch_keep(bf16, std::integral_constant<int, 3>{});
+      case 4: return launch_keep(bf16, std::integral_constant<int, 4>{});
+      case 5: return launch_keep(bf16, std::integral_constant<int, 5>{});
+      case 6: return launch_keep(bf16, std::integral_constant<int, 6>{});
+      case 7: return launch_keep(bf16, std::integral_constant<int, 7>{});
+      default: return launch_keep(bf16, std::integral_constant<int, 8>{});
+    }
   };
   return x_dtype == QGEMM_DT_BF16 ? launch_type(std::true_type{}) : launch_type(std::false_type{});
 }

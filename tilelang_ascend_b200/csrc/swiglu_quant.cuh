@@ -3,11 +3,16 @@
 //   a = g / (1 + exp(-g)) * u          s = RN32(max(max|a|, 1e-4) / 127)  (round_scale: the power of two not below it)
 //   y = the integer nearest to a / s
 //
-// y and s are those of the exact a, so that they depend on no implementation's rounding of exp: fp32 values decide all but
-// the elements next to a border, which are taken again in fp64 - the candidates for the row's largest value, a few per row, and the
-// quotients within SQ_NEAR of a half, about one in 3000.  (For |u| < 1e26 where g < -80: below that exp leaves fp32's normal range.)
+// y and s are those of the exact a, so that they depend on no implementation's rounding of exp.  fp32 values decide all but
+// the elements next to a border, which are taken again in fp64: the candidates for the row's largest value, one or two per row, and the
+// quotients that lie as near to n + 1/2 as fp32 may be wrong, one in 1000 or so.
 //
-// 4 F bytes in and F out per row.
+// What fp32 makes of a, relative: 2^-22 by ex2.approx, |g| 7.5e-8 by the rounding of its argument where g < 0 (where g > 0 the factor
+// e / (1 + e) takes it down to 2e-8), 2^-24 by the sum, 2^-23 by rcp.approx, 2^-23 by two products: 5.4e-7 + 7.5e-8 max(0, -g).  The
+// quotient by s adds 2.4e-7.  (For g < -87 fp32 gives 0 where a is up to 1e-36 |u|: right as long as |u| < 1e29.)
+//
+// 4 F bytes in and F out per row.  A row is held in registers as fp32 between its maximum and its codes.  Pairs of values go through
+// the packed fp32 instructions; two MUFU operations per element are the next bound behind memory.
 #pragma once
 
 #include "act_quant.cuh"
@@ -24,133 +29,268 @@ struct SwigluQuantParams {
   int round_scale;
 };
 
-// What fp32 makes of a: exp to 2 ulp, the quotient to 2, and three roundings, 6.6e-7 in all; times 127 with the two roundings of the
-// quotient by s, 9.8e-5 of a step.
-constexpr float SQ_NEAR = 1.5e-4f;
-constexpr float SQ_TOP = 1.0f - 0x1p-18f;  // whoever is this near to the fp32 maximum may be the largest
+// ------------------------------------------------------------------------ two fp32 values in a 64-bit register
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 f2_make(float lo, float hi) {
+  f32x2 v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
+  return v;
+}
+__device__ __forceinline__ void f2_get(f32x2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+__device__ __forceinline__ f32x2 f2_mul(f32x2 a, f32x2 b) {
+  f32x2 v;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ f32x2 f2_add(f32x2 a, f32x2 b) {
+  f32x2 v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+__device__ __forceinline__ f32x2 f2_fma(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+// The largest of three absolute values; NaN if one is.
+__device__ __forceinline__ float f3_max_abs(float a, float b, float c) {
+  float v;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
+  return v;
+}
+template <bool BF16>
+__device__ __forceinline__ f32x2 f2_of_half2(uint32_t w) {
+  if constexpr (BF16) return f2_make(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return f2_make(f.x, f.y);
+}
 
-__device__ __forceinline__ float sq_gate(float g, float u) {
-  const float e = expf(-fabsf(g));  // at most 1, so that nothing overflows
-  return __fdividef(g < 0.0f ? g * e : g, 1.0f + e) * u;
+// --------------------------------------------------------------------------------------------------- a in fp32 and fp64
+__device__ __forceinline__ float sq_exp2(float t) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  return e;
+}
+__device__ __forceinline__ float sq_rcp(float d) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  return r;
+}
+__device__ __forceinline__ f32x2 sq_gate(f32x2 g, f32x2 u) {
+  const float L = -1.4426950408889634f;  // -log2(e)
+  float t0, t1, d0, d1;
+  f2_get(f2_mul(g, f2_make(L, L)), t0, t1);
+  f2_get(f2_add(f2_make(sq_exp2(t0), sq_exp2(t1)), f2_make(1.0f, 1.0f)), d0, d1);
+  return f2_mul(f2_mul(g, f2_make(sq_rcp(d0), sq_rcp(d1))), u);
+}
+template <bool BF16>
+__device__ __forceinline__ float sq_float(uint32_t bits) {
+  if constexpr (BF16) return __uint_as_float(bits << 16);
+  return __half2float(__ushort_as_half((unsigned short)bits));
+}
+template <bool BF16>
+__device__ __forceinline__ float sq_element(const uint4* p, int i) {
+  return sq_float<BF16>(*(reinterpret_cast<const volatile uint16_t*>(p) + i));
 }
 __device__ __forceinline__ double sq_gate64(float g, float u) { return (double)g / (1.0 + exp(-(double)g)) * (double)u; }
 
 template <bool BF16>
-__device__ __forceinline__ float sq_element(const void* p, long long i) {
-  uint16_t h;
-  asm volatile("ld.global.u16 %0, [%1];" : "=h"(h) : "l"(static_cast<const uint16_t*>(p) + i));
-  if constexpr (BF16) return __uint_as_float((uint32_t)h << 16);
-  return __half2float(__ushort_as_half(h));
+__device__ __forceinline__ void sq_gate8(const uint4& g, const uint4& u, f32x2 (&a)[4]) {
+  const uint32_t gw[4] = {g.x, g.y, g.z, g.w}, uw[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) a[i] = sq_gate(f2_of_half2<BF16>(gw[i]), f2_of_half2<BF16>(uw[i]));
 }
 
-// |a| of the elements of chunk c that may be the row's largest, in fp64.
+// The elements of a chunk that are marked, in fp64: the largest |a| of them ...
 template <bool BF16>
-__device__ __noinline__ double sq_largest64(const uint4* x, int chunks, int c, float from) {
+__device__ __noinline__ double sq_largest64(const uint4* gp, const uint4* up, uint32_t marked) {
   double best = 0.0;
-  for (int i = 0; i < 8; ++i) {
-    const float g = sq_element<BF16>(x, 8ll * c + i), u = sq_element<BF16>(x, 8ll * (chunks + c) + i);
-    if (fabsf(sq_gate(g, u)) >= from) best = fmax(best, fabs(sq_gate64(g, u)));
+  for (; marked != 0; marked &= marked - 1) {
+    const int i = __ffs(marked) - 1;
+    best = fmax(best, fabs(sq_gate64(sq_element<BF16>(gp, i), sq_element<BF16>(up, i))));
   }
   return best;
 }
-// The codes of the marked elements of chunk c in fp64.
+// ... and their codes, which take the place of those that fp32 gave.
 template <bool BF16>
-__device__ __noinline__ uint2 sq_codes64(const uint4* x, int chunks, int c, float scale, uint32_t marked, uint2 codes) {
-  for (int i = 0; i < 8; ++i) {
-    if (!((marked >> i) & 1u)) continue;
-    const float g = sq_element<BF16>(x, 8ll * c + i), u = sq_element<BF16>(x, 8ll * (chunks + c) + i);
-    const double q = fmin(fmax(rint(sq_gate64(g, u) / (double)scale), -127.0), 127.0);
-    const uint32_t code = (uint32_t)(int)q & 0xffu, at = 8u * (i & 3);
+__device__ __noinline__ uint2 sq_codes64(const uint4* gp, const uint4* up, float scale, uint32_t marked, uint2 codes) {
+  for (; marked != 0; marked &= marked - 1) {
+    const int i = __ffs(marked) - 1;
+    const double q = sq_gate64(sq_element<BF16>(gp, i), sq_element<BF16>(up, i)) / (double)scale;
+    const uint32_t code = (uint32_t)__double2int_rn(fmin(fmax(q, -127.0), 127.0)) & 0xffu, at = 8u * (i & 3);
     uint32_t& w = i < 4 ? codes.x : codes.y;
     w = (w & ~(0xffu << at)) | (code << at);
   }
   return codes;
 }
 
-template <bool BF16>
-__device__ __forceinline__ void sq_gate8(const uint4& g, const uint4& u, float (&a)[8]) {
-  float gf[8], uf[8];
-  aq_unpack8(g, BF16, gf);
-  aq_unpack8(u, BF16, uf);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) a[i] = sq_gate(gf[i], uf[i]);
+// TPR threads share a row, KEEP chunks of eight elements of it in each one's registers; longer rows are computed again for their codes.
+// The blocks are persistent: the next row's loads are issued when this one's values are in fp32, and are in flight while its
+// maximum is settled and its codes are stored.
+__host__ __device__ constexpr int sq_block(int tpr) { return tpr == 32 ? 128 : tpr; }
+// Blocks per SM that the registers have to allow: 384 threads where a warp has a row to itself, otherwise 512 at five chunks and more,
+// so that another row goes on while one waits for its two barriers.  us, 128 registers / the compiler's 168 - 180: 5000 x 7168
+// 43.5 / 46.5, 4000 x 14336 81 / 100, but 32768 x 2048 64.5 / 62.9.
+__host__ __device__ constexpr int sq_min_blocks(int tpr, int keep) {
+  const int threads = keep > 4 ? (tpr == 32 ? 384 : 512) : keep > 2 ? 640 : keep == 2 ? 768 : 1024;
+  return threads / sq_block(tpr) > 0 ? threads / sq_block(tpr) : 1;
 }
-
+__host__ __device__ constexpr int sq_smem_bytes(int tpr, int keep) { return keep * 32 * sq_block(tpr); }
 template <int TPR, int KEEP, bool BF16>
-__global__ void __launch_bounds__(aq_block(TPR)) swiglu_quant_kernel(const SwigluQuantParams p) {
+__global__ void __launch_bounds__(sq_block(TPR), sq_min_blocks(TPR, KEEP)) swiglu_quant_kernel(const SwigluQuantParams p) {
   pdl_wait();
   pdl_launch_dependents();
-  constexpr int ROWS = aq_block(TPR) / TPR;
+  constexpr int ROWS = sq_block(TPR) / TPR;
   constexpr int WPR = TPR / 32;  // warps per row
-  __shared__ uint32_t red[aq_block(TPR) / 32];
-  __shared__ unsigned long long largest[ROWS];
+  static_assert(WPR == 1 || ROWS == 1, "barriers are of the whole block");
+  __shared__ uint32_t red[2][WPR];
+  __shared__ uint32_t largest[2];  // scales as bits, of this row and the next one
   const int t = threadIdx.x % TPR;
-  const int r = threadIdx.x / TPR;
   const int warp = threadIdx.x >> 5;
-  const long long row = (long long)blockIdx.x * ROWS + r;
-  const bool live = row < p.M;
   const int chunks = p.F >> 3;
-  const uint4* x = p.X + (live ? row : 0) * 2 * chunks;
-  if (t == 0) largest[r] = 0ull;
-
-  float a[KEEP][8];
-  uint32_t m = 0;  // |a| as an integer: the same order, with inf and NaN on top
-  auto take = [&](int c, float (&v)[8]) {
-    sq_gate8<BF16>(ld_written(x + c), ld_written(x + chunks + c), v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-  };
-  if (live) {
-#pragma unroll
-    for (int i = 0; i < KEEP; ++i)
-      if (t + i * TPR < chunks) take(t + i * TPR, a[i]);
-    for (int c = t + KEEP * TPR; c < chunks; c += TPR) {
-      float v[8];
-      take(c, v);
-    }
-  }
-  const uint32_t own = m;
-  m = __reduce_max_sync(0xffffffffu, m);
-  if ((threadIdx.x & 31) == 0) red[warp] = m;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < WPR; ++w) m = max(m, red[r * WPR + w]);
-  const bool finite = m < 0x7f800000u;
-  const float from = __uint_as_float(m) * SQ_TOP;
-  if (live && finite && m != 0 && __uint_as_float(own) >= from) {
-    double best = 0.0;
-    for (int c = t; c < chunks; c += TPR) best = fmax(best, sq_largest64<BF16>(x, chunks, c, from));
-    atomicMax(&largest[r], (unsigned long long)__double_as_longlong(best));
-  }
-  __syncthreads();
-  float scale = (float)(fmax(__longlong_as_double((long long)largest[r]), 1e-4) / 127.0);
-  if (p.round_scale) scale = aq_pow2_ceil(scale);
-  if (!finite) scale = __uint_as_float(m);  // inf or NaN: it stays one
-  if (!live) return;
-  if (t == 0) p.S[row] = scale;
-  const float rcp = __frcp_rn(scale);
-  uint2* y = reinterpret_cast<uint2*>(p.Y) + row * chunks;
-  auto store = [&](int c, const float (&v)[8]) {
-    const float MAGIC = 12582912.0f;  // 1.5 * 2^23: the sum's low bits are the nearest integer
-    float f[8];
-    uint32_t marked = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float q = v[i] * rcp;
-      f[i] = q + MAGIC;
-      if (fabsf(q - (f[i] - MAGIC)) > 0.5f - SQ_NEAR) marked |= 1u << i;
-    }
-    uint2 codes = make_uint2(aq_pack4(f), aq_pack4(f + 4));
-    if (marked) codes = sq_codes64<BF16>(x, chunks, c, scale, marked, codes);
-    y[c] = codes;
-  };
+  const long long step = (long long)gridDim.x * ROWS;
+  long long row = (long long)blockIdx.x * ROWS + threadIdx.x / TPR;
+  if (WPR > 1 && t == 0) largest[0] = 0u;
+  // a thread copies its own chunks into its own slots, so that no barrier is needed to read them
+  extern __shared__ uint4 sq_slots[];
+  uint4* slot = sq_slots + threadIdx.x;  // gate chunk i: slot[2 i block], up chunk i: slot[(2 i + 1) block]
+  constexpr int BLOCK = sq_block(TPR);
 #pragma unroll
   for (int i = 0; i < KEEP; ++i)
-    if (t + i * TPR < chunks) store(t + i * TPR, a[i]);
-  for (int c = t + KEEP * TPR; c < chunks; c += TPR) {
-    float v[8];
-    sq_gate8<BF16>(ld_written(x + c), ld_written(x + chunks + c), v);
-    store(c, v);
+    if (t + i * TPR >= chunks) slot[2 * i * BLOCK] = slot[(2 * i + 1) * BLOCK] = make_uint4(0u, 0u, 0u, 0u);
+  auto load = [&](long long of) {
+    const uint4* x = p.X + of * 2 * chunks;
+    if (of < p.M) {
+#pragma unroll
+      for (int i = 0; i < KEEP; ++i) {
+        const int c = t + i * TPR;
+        if (c < chunks) {
+          cp_async16(smem_u32(slot + 2 * i * BLOCK), x + c);
+          cp_async16(smem_u32(slot + (2 * i + 1) * BLOCK), x + chunks + c);
+        }
+      }
+    }
+  };
+  load(row);
+  const f32x2 magic = f2_make(12582912.0f, 12582912.0f), unmagic = f2_make(-12582912.0f, -12582912.0f);
+  for (int turn = 0; row < p.M; row += step, turn ^= 1) {
+    const uint4* x = p.X + row * 2 * chunks;
+    f32x2 a[KEEP][4];
+    float most[KEEP], top = 0.0f;  // |a|: of a chunk, of this thread
+    uint32_t low2 = 0;             // the lowest gates of this thread, as bits: negative numbers are the larger the lower they are
+    auto take = [&](const uint4& gc, const uint4& uc, f32x2 (&v)[4]) {
+      low2 = __vimax3_u16x2(__vimax3_u16x2(low2, gc.x, gc.y), gc.z, gc.w);
+      sq_gate8<BF16>(gc, uc, v);
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f2_get(v[i], f[2 * i], f[2 * i + 1]);
+      return f3_max_abs(f3_max_abs(f[0], f[1], f[2]), f3_max_abs(f[3], f[4], f[5]), f3_max_abs(f[6], f[7], 0.0f));
+    };
+    cp_async_wait();
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i) most[i] = take(slot[2 * i * BLOCK], slot[(2 * i + 1) * BLOCK], a[i]);
+#pragma unroll
+    for (int i = 0; i < KEEP; i += 2) top = f3_max_abs(top, most[i], most[i + 1 < KEEP ? i + 1 : i]);
+    for (int c = t + KEEP * TPR; c < chunks; c += TPR) {
+      f32x2 v[4];
+      top = f3_max_abs(top, take(ld_written(x + c), ld_written(x + chunks + c), v), 0.0f);
+    }
+    uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(top) & 0x7fffffffu);  // as integers NaN and inf are on top
+    uint32_t low = __reduce_max_sync(0xffffffffu, max(low2 & 0xffffu, low2 >> 16));
+    if (WPR > 1) {
+      if ((threadIdx.x & 31) == 0) {
+        red[0][warp] = m;
+        red[1][warp] = low;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < WPR; ++w) {
+        m = max(m, red[0][w]);
+        low = max(low, red[1][w]);
+      }
+      if (t == 0) largest[turn ^ 1] = 0u;  // everybody is through with the last row's
+    }
+    const bool finite = m < 0x7f800000u;
+    float lowest = 0.0f;  // max(0, -g) over the row; beyond 88 fp32 gives 0 for a
+    if (low & 0x8000u) lowest = fminf(BF16 ? __uint_as_float((low & 0x7fffu) << 16) : __half2float(__ushort_as_half((unsigned short)(low & 0x7fffu))), 88.0f);
+    const float off = 5.5e-7f + 7.5e-8f * lowest;
+    const float from = __uint_as_float(m) * (1.0f - (2.0f * off + 2e-7f));
+    double best = 0.0;
+    // Whoever may be the largest: nearly always one element of one thread, whose gate and up are kept over the next row's loads.
+    uint32_t only = 0, only_g = 0, only_u = 0;
+    const bool may = finite && m != 0 && top >= from;
+    if (may) {
+      auto consider = [&](const uint4* gp, const uint4* up, const f32x2 (&v)[4]) {
+        uint32_t marked = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float lo, hi;
+          f2_get(v[i], lo, hi);
+          marked |= (fabsf(lo) >= from ? 1u << (2 * i) : 0u) | (fabsf(hi) >= from ? 2u << (2 * i) : 0u);
+        }
+        if (only == 0 && (marked & (marked - 1)) == 0) {
+          only = marked;
+          const int i = __ffs(marked) - 1;
+          only_g = reinterpret_cast<const volatile uint16_t*>(gp)[i];
+          only_u = reinterpret_cast<const volatile uint16_t*>(up)[i];
+        } else {
+          best = fmax(best, sq_largest64<BF16>(gp, up, marked));
+        }
+      };
+#pragma unroll
+      for (int i = 0; i < KEEP; ++i)
+        if (most[i] >= from) consider(slot + 2 * i * BLOCK, slot + (2 * i + 1) * BLOCK, a[i]);
+      for (int c = t + KEEP * TPR; c < chunks; c += TPR) {
+        f32x2 v[4];
+        const float most_here = take(ld_written(x + c), ld_written(x + chunks + c), v);
+        if (most_here >= from) consider(x + c, x + chunks + c, v);
+      }
+    }
+    load(row + step);  // every slot has been read
+    if (only != 0) best = fmax(best, fabs(sq_gate64(sq_float<BF16>(only_g), sq_float<BF16>(only_u))));
+    // The scale of each candidate, as bits; rounding keeps the order, so that the largest is the row's.
+    uint32_t bits = __float_as_uint((float)(fmax(best, 1e-4) * (1.0 / 127.0)));
+    if (WPR > 1) {
+      if (may) atomicMax(&largest[turn], bits);
+      __syncthreads();
+      bits = max(bits, largest[turn]);
+    } else {
+      bits = __reduce_max_sync(0xffffffffu, bits);
+    }
+    float scale = __uint_as_float(bits);
+    if (p.round_scale) scale = aq_pow2_ceil(scale);
+    if (!finite) scale = __uint_as_float(m);  // inf or NaN: it stays one
+    if (t == 0) p.S[row] = scale;
+    const float rcp = sq_rcp(scale);
+    const float share = finite ? rcp * (off + 2.5e-7f) : 0.0f;  // what a quotient may be off by, per |a|
+    uint2* y = reinterpret_cast<uint2*>(p.Y) + row * chunks;
+    const f32x2 rcp2 = f2_make(rcp, rcp), less_rcp2 = f2_make(-rcp, -rcp);
+    auto store = [&](int c, const f32x2 (&v)[4], float m) {
+      float f[8], d[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x2 s = f2_fma(v[i], rcp2, magic);  // 1.5 * 2^23 + a / s: the low bits are the nearest integer
+        f2_get(s, f[2 * i], f[2 * i + 1]);
+        f2_get(f2_fma(v[i], less_rcp2, f2_add(s, unmagic)), d[2 * i], d[2 * i + 1]);  // how far it is
+      }
+      uint2 codes = make_uint2(aq_pack4(f), aq_pack4(f + 4));
+      const float sure = 0.5f - m * share;
+      if (f3_max_abs(f3_max_abs(d[0], d[1], d[2]), f3_max_abs(d[3], d[4], d[5]), f3_max_abs(d[6], d[7], 0.0f)) > sure) {
+        uint32_t marked = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) marked |= fabsf(d[i]) > sure ? 1u << i : 0u;
+        codes = sq_codes64<BF16>(x + c, x + chunks + c, scale, marked, codes);
+      }
+      y[c] = codes;
+    };
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+      if (t + i * TPR < chunks) store(t + i * TPR, a[i], most[i]);
+    for (int c = t + KEEP * TPR; c < chunks; c += TPR) {
+      f32x2 v[4];
+      sq_gate8<BF16>(ld_written(x + c), ld_written(x + chunks + c), v);
+      store(c, v, __uint_as_float(m));
+    }
   }
 }
 
