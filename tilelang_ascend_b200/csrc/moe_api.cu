@@ -39,17 +39,26 @@ int launch_swiglu(const qg::SwigluQuantParams& p, int sms, cudaStream_t s) {
   return launch_pdl(kernel, (int)grid, block, smem, s, p);
 }
 
+template <int DT, bool VEC>
+int launch_route(const qg::MoeRouteParams& p, int sms, cudaStream_t s) {
+  const long long blocks = std::min<long long>((p.T + qg::RT_WARPS - 1) / qg::RT_WARPS, 8ll * sms);
+  const int smem = qg::rt_smem_bytes(p.E);
+  auto launch = [&](auto kernel) { return launch_pdl(kernel, (int)blocks, qg::RT_WARPS * 32, smem, s, p); };
+  if (p.E <= 32) return launch(qg::moe_route_kernel<DT, 1, VEC>);
+  if (p.E <= 64) return launch(qg::moe_route_kernel<DT, 2, VEC>);
+  if (p.E <= 128) return launch(qg::moe_route_kernel<DT, 4, VEC>);
+  if (p.E <= 256) return launch(qg::moe_route_kernel<DT, 8, VEC>);
+  if (p.E <= 512) return launch(qg::moe_route_kernel<DT, 16, VEC>);
+  return launch(qg::moe_route_kernel<DT, 32, VEC>);
+}
 template <int DT>
 int launch_route(const qg::MoeRouteParams& p, int sms, cudaStream_t s) {
-  const long long blocks = std::min<long long>((p.T + qg::RT_WARPS - 1) / qg::RT_WARPS, 16ll * sms);
-  const int smem = qg::RT_WARPS * 8 * p.E;
-  auto launch = [&](auto kernel) { return launch_pdl(kernel, (int)blocks, qg::RT_WARPS * 32, smem, s, p); };
-  if (p.E <= 32) return launch(qg::moe_route_kernel<DT, 1>);
-  if (p.E <= 64) return launch(qg::moe_route_kernel<DT, 2>);
-  if (p.E <= 128) return launch(qg::moe_route_kernel<DT, 4>);
-  if (p.E <= 256) return launch(qg::moe_route_kernel<DT, 8>);
-  if (p.E <= 512) return launch(qg::moe_route_kernel<DT, 16>);
-  return launch(qg::moe_route_kernel<DT, 32>);
+  // A lane's logits in pieces of up to 16 bytes where every row keeps that alignment and no lane has some of its experts only.
+  int v = 1;
+  while (32 * v < p.E) v *= 2;
+  const int bytes = std::min(16, v * (DT == qg::RT_F32 ? 4 : 2));
+  const bool vec = p.E % v == 0 && (int64_t)p.E * (DT == qg::RT_F32 ? 4 : 2) % bytes == 0 && aligned(p.logits, bytes);
+  return vec ? launch_route<DT, true>(p, sms, s) : launch_route<DT, false>(p, sms, s);
 }
 
 // Once per device: the block-table kernel's shared memory and its clusters of more than eight CTAs.

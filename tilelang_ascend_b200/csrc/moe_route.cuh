@@ -7,9 +7,13 @@
 //
 // The picks are those of the real numbers: two scores that fp32 cannot tell apart must not depend on how a kernel adds.  Without
 // a bias the logits themselves are compared (both score functions are increasing).  With one, or with sums of two scores, fp32
-// values are compared and a token whose decision is nearer than the error of the fp32 scores is decided again in fp64.
+// values are compared and a token whose decision is nearer than the error of the fp32 scores is decided again in fp64 (random
+// scores: one token in some hundreds).
 //
-// One warp per token, experts dealt to the lanes (lane + 32 i), in registers.
+// One warp per token.  A lane has V consecutive experts as 32-bit keys in the order of the values, whose lowest bits are the place within
+// the lane, and sorts them (in lists of eight) in registers.  A pick is then a maximum over the lanes' heads, one redux instruction, and a
+// step of the winning lane's list: 14 instructions where a search of all values for the maximum would be 40.  E 4 bytes of
+// reading per token are 300 - 400 instructions of a warp, which is what bounds it: 16384 x 256 is 1.5 us of memory and 5 of issue.
 #pragma once
 
 #include "common.cuh"
@@ -54,13 +58,16 @@ __device__ __forceinline__ float rt_max(float a, float b) {
 }
 
 // Values as unsigned numbers of the same order; NaN above everything, both zeros alike, -inf (not offered) at RT_NONE.
+constexpr int RT_LIST = 68;  // two lists of 34 entries of a warp, on a 16-byte boundary
+__host__ __device__ constexpr int rt_smem_bytes(int E) { return 8 * (RT_WARPS * E + (RT_WARPS * E & 1) + RT_WARPS * RT_LIST); }
+
 template <typename K> struct RtKey;
 template <> struct RtKey<uint32_t> {
   using F = float;
   static constexpr uint32_t NONE = 0x007fffffu;
   static __device__ __forceinline__ uint32_t of(float v) {
-    const uint32_t b = __float_as_uint(v + 0.0f);
-    return v != v ? 0xffffffffu : b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
+    const uint32_t b = __float_as_uint(v + 0.0f);  // (a NaN comes out of an addition as 0x7fffffff)
+    return b ^ ((uint32_t)((int)b >> 31) | 0x80000000u);
   }
   static __device__ __forceinline__ float value(uint32_t k) {
     return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
@@ -84,10 +91,29 @@ template <> struct RtKey<unsigned long long> {
   }
 };
 
+// What a group with the largest keys a and b is worth.  Keys of logits stand for their scores, for softmax times a common factor.
+template <typename F, typename K>
+__device__ __forceinline__ F rt_group_value(const MoeRouteParams& p, K a, K b, bool by_logits, float top) {
+  F v = RtKey<K>::value(a > RtKey<K>::NONE ? a : RtKey<K>::NONE);
+  if (p.group_top == 1) return v;
+  F w = RtKey<K>::value(b > RtKey<K>::NONE ? b : RtKey<K>::NONE);
+  if (by_logits && a > RtKey<K>::NONE) {
+    auto score = [&](F l) -> F {
+      if constexpr (sizeof(F) == 8) return p.softmax ? exp(l - (F)top) : 1.0 / (1.0 + exp(-l));
+      else return p.softmax ? expf(l - top) : __fdividef(1.0f, 1.0f + expf(-l));
+    };
+    v = score(v);
+    w = b > RtKey<K>::NONE ? score(w) : w;
+  }
+  return b > RtKey<K>::NONE ? v + w : v;
+}
+
 // The groups that stay, as a bit mask.  `keys`: this warp's c in shared memory.  P lanes share a group and keep its two largest
-// keys.  `eps` >= 0: `near` is set where the border between the groups that stay and the others is no wider than the error of c.
+// keys.  `eps` >= 0: `near` is set where the last
+// group that stays and the first that does not are no further apart than two sums of two c that may each be off by half of that.
 template <typename K>
-__device__ __forceinline__ uint32_t rt_groups(const MoeRouteParams& p, const K* keys, int lane, typename RtKey<K>::F eps, bool& near) {
+__device__ __forceinline__ uint32_t rt_groups(const MoeRouteParams& p, const K* keys, int lane, bool by_logits, float top,
+                                              typename RtKey<K>::F eps, bool& near) {
   using F = typename RtKey<K>::F;
   int share = 1;
   while (share * 2 * p.groups <= 32) share *= 2;
@@ -106,8 +132,7 @@ __device__ __forceinline__ uint32_t rt_groups(const MoeRouteParams& p, const K* 
     a = a > a2 ? a : a2;
     b = lo > hi2 ? lo : hi2;
   }
-  F v = RtKey<K>::value(a > RtKey<K>::NONE ? a : RtKey<K>::NONE);
-  if (p.group_top == 2 && b > RtKey<K>::NONE) v += RtKey<K>::value(b);
+  const F v = rt_group_value<F>(p, a, b, by_logits, top);
   const K mine = g < p.groups ? RtKey<K>::of(v) : 0;
   int rank = 0;
   for (int j = 0; j < p.groups; ++j) {
@@ -115,11 +140,11 @@ __device__ __forceinline__ uint32_t rt_groups(const MoeRouteParams& p, const K* 
     rank += (other > mine || (other == mine && j < g)) ? 1 : 0;
   }
   const bool leads = part == 0 && g < p.groups;
-  if (eps >= 0 && p.top_groups < p.groups) {
+  if (eps >= 0 && !(by_logits && p.group_top == 1)) {
     const uint32_t last = __ballot_sync(0xffffffffu, leads && rank == p.top_groups - 1);
     const uint32_t next = __ballot_sync(0xffffffffu, leads && rank == p.top_groups);
     const F x = __shfl_sync(0xffffffffu, v, __ffs(last) - 1), y = __shfl_sync(0xffffffffu, v, __ffs(next) - 1);
-    if (x - y <= 2 * eps + (F)0x1p-21 * (fabs(x) + fabs(y))) near = true;
+    if (x - y <= 2 * eps) near = true;
   }
   uint32_t stays = 0;
   const uint32_t kept = __ballot_sync(0xffffffffu, leads && rank < p.top_groups);
@@ -127,164 +152,452 @@ __device__ __forceinline__ uint32_t rt_groups(const MoeRouteParams& p, const K* 
   return stays;
 }
 
-// One token again in fp64; lane j < k returns pick j or -1.
-__device__ __noinline__ int rt_decide_in_64(const MoeRouteParams& p, const void* row, int dt, unsigned long long* keys, bool by_logits,
-                                            float top, int lane) {
-  using K = RtKey<unsigned long long>;
-  auto logit = [&](int e) { return dt == RT_F32 ? rt_load<RT_F32>(row, e) : dt == RT_BF16 ? rt_load<RT_BF16>(row, e) : rt_load<RT_F16>(row, e); };
-  double sum = 0;
-  if (p.softmax) {
+// What is compared, in fp64: without a bias the exact logits.
+struct RtScore64 {
+  const MoeRouteParams& p;
+  const void* row;
+  int dt;
+  bool by_logits;
+  float top = 0.0f;
+  double sum = 1.0;
+  __device__ __forceinline__ float logit(int e) const {
+    return dt == RT_F32 ? rt_load<RT_F32>(row, e) : dt == RT_BF16 ? rt_load<RT_BF16>(row, e) : rt_load<RT_F16>(row, e);
+  }
+  __device__ __forceinline__ void prepare(int lane) {
+    uint32_t most = 0;
+    for (int e = lane; e < p.E; e += 32) most = max(most, RtKey<uint32_t>::of(logit(e)));
+    top = RtKey<uint32_t>::value(RtKey<uint32_t>::warp_max(most));
+    if (!p.softmax || by_logits) return;
+    sum = 0.0;
     for (int e = lane; e < p.E; e += 32) sum += exp((double)logit(e) - (double)top);
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
-  auto fill = [&](bool logits) {
-    __syncwarp();
-    for (int e = lane; e < p.E; e += 32) {
-      const float l = logit(e);
-      double c = (double)l;
-      if (!logits) {
-        c = p.softmax ? exp((double)l - (double)top) / sum : 1.0 / (1.0 + exp(-(double)l));
-        if (p.bias != nullptr) c += (double)ld_written(p.bias + e);
-        if (l == -INFINITY) c = -INFINITY;
-      }
-      keys[e] = K::of(c);
+  __device__ __forceinline__ unsigned long long key(int e) const {
+    const float l = logit(e);
+    double c = (double)l;
+    if (!by_logits) {
+      c = (p.softmax ? exp((double)l - (double)top) / sum : 1.0 / (1.0 + exp(-(double)l))) + (double)ld_written(p.bias + e);
+      if (l == -INFINITY) c = -INFINITY;
     }
-    __syncwarp();
-  };
-  fill(false);
+    return RtKey<unsigned long long>::of(c);
+  }
+};
+
+// One token again in fp64; lane j < k returns pick j or -1.
+__device__ __noinline__ int rt_decide_in_64(const MoeRouteParams& p, const void* row, int dt, unsigned long long* keys, bool by_logits, int lane) {
+  using K = RtKey<unsigned long long>;
+  RtScore64 score{p, row, dt, by_logits};
+  score.prepare(lane);
+  __syncwarp();
+  for (int e = lane; e < p.E; e += 32) keys[e] = score.key(e);
+  __syncwarp();
   bool near = false;
-  uint32_t stays = 0xffffffffu;
-  if (p.groups > 1) stays = rt_groups<unsigned long long>(p, keys, lane, -1.0, near);
-  if (by_logits) fill(true);
+  if (p.groups > 1) {
+    const uint32_t stays = rt_groups<unsigned long long>(p, keys, lane, by_logits, score.top, -1.0, near);
+    __syncwarp();
+    for (int e = lane; e < p.E; e += 32)
+      if (!((stays >> (e / p.group_n)) & 1u)) keys[e] = 0;
+  }
   int pick = -1;
   for (int r = 0; r < p.k; ++r) {
+    __syncwarp();
     unsigned long long best = 0;
     int at = 0x7fffffff;
-    for (int e = lane; e < p.E; e += 32)
-      if (((stays >> (e / p.group_n)) & 1u) && keys[e] > best) { best = keys[e]; at = e; }
+    for (int e = lane; e < p.E; e += 32) {
+      const unsigned long long k = keys[e];
+      if (k > best) { best = k; at = e; }
+    }
     const unsigned long long m = K::warp_max(best);
     if (m <= K::NONE) break;
     const int e = __reduce_min_sync(0xffffffffu, best == m ? at : 0x7fffffff);
     if (lane == r) pick = e;
-    __syncwarp();
-    if (lane == 0) keys[e] = 0;
-    __syncwarp();
+    if (lane == (e & 31)) keys[e] = 0;
   }
   return pick;
 }
 
-template <int DT, int V>
+// The order of n candidates, expert `e` of lane < n, in fp64.
+__device__ __noinline__ int rt_rank_in_64(const MoeRouteParams& p, const void* row, int dt, bool by_logits, int e, int n, int lane) {
+  RtScore64 score{p, row, dt, by_logits};
+  if (p.softmax && !by_logits) score.prepare(lane);
+  const unsigned long long mine = lane < n ? score.key(e) : 0ull;
+  int rank = 0;
+  for (int i = 0; i < n; ++i) {
+    const unsigned long long other = __shfl_sync(0xffffffffu, mine, i);
+    const int f = __shfl_sync(0xffffffffu, e, i);
+    rank += other > mine || (other == mine && f < e) ? 1 : 0;
+  }
+  return lane < n ? rank : lane;
+}
+
+__device__ __forceinline__ float rt_exp2(float t) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  return e;
+}
+__device__ __forceinline__ float rt_rcp(float d) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  return r;
+}
+constexpr float RT_LOG2E = 1.4426950408889634f;
+// Off by less than 2^-21: the error of exp, 2^-22 + |l| 7.5e-8, enters times s (1 - s), and sum and reciprocal add 1.5 * 2^-23.
+__device__ __forceinline__ float rt_sigmoid(float l) { return rt_rcp(1.0f + rt_exp2(-RT_LOG2E * l)); }
+// exp(l - top) to 2^-22 + |l - top| 7.5e-8, relative: the argument's rounding is put right behind the approximation.
+__device__ __forceinline__ float rt_exp_below(float l, float top) {
+  const float x = l - top, t = x * RT_LOG2E, e = rt_exp2(t);
+  return x < -100.0f ? 0.0f : fmaf(e, fmaf(x, RT_LOG2E, -t) * 0.6931471806f, e);
+}
+
+// Largest first.
+template <int L>
+__device__ __forceinline__ void rt_sort(uint32_t (&k)[L]) {
+  auto order = [&](int i, int j) {
+    const uint32_t hi = max(k[i], k[j]), lo = min(k[i], k[j]);
+    k[i] = hi;
+    k[j] = lo;
+  };
+  if constexpr (L == 2) {
+    order(0, 1);
+  } else if constexpr (L == 4) {
+    order(0, 1), order(2, 3), order(0, 2), order(1, 3), order(1, 2);
+  } else if constexpr (L == 8) {
+    order(0, 2), order(1, 3), order(4, 6), order(5, 7), order(0, 4), order(1, 5), order(2, 6), order(3, 7), order(0, 1), order(2, 3);
+    order(4, 5), order(6, 7), order(2, 4), order(3, 5), order(1, 4), order(3, 6), order(1, 2), order(3, 4), order(5, 6);
+  }
+}
+
+// A lane's V logits, by loads of up to 16 bytes (VEC: every lane has all V or none, and rows keep the alignment) or one by one.
+template <int DT, int V, bool VEC>
+struct RtRow {
+  static constexpr int BYTES = V * (DT == RT_F32 ? 4 : 2);
+  static constexpr int WORDS = VEC ? (BYTES + 3) / 4 : V;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ RtRow() {  // -inf, which a lane without experts keeps
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) w[i] = !VEC || DT == RT_F32 ? 0xff800000u : (DT == RT_BF16 ? 0xff80ff80u : 0xfc00fc00u);
+  }
+  __device__ __forceinline__ void load(const void* row, int first, int E) {
+    const char* p = static_cast<const char*>(row) + (long long)first * (DT == RT_F32 ? 4 : 2);
+    if constexpr (!VEC) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) w[i] = first + i < E ? __float_as_uint(rt_load<DT>(row, first + i)) : 0xff800000u;
+    } else {
+      if (first >= E) return;
+      if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+        for (int i = 0; i < BYTES / 16; ++i) {
+          const uint4 v = ld_written(reinterpret_cast<const uint4*>(p) + i);
+          w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+        }
+      } else if constexpr (BYTES == 8) {
+        const uint2 v = ld_written(reinterpret_cast<const uint2*>(p));
+        w[0] = v.x, w[1] = v.y;
+      } else if constexpr (BYTES == 4) {
+        w[0] = (uint32_t)ld_written(reinterpret_cast<const int*>(p));
+      } else {
+        uint16_t h;
+        asm volatile("ld.global.u16 %0, [%1];" : "=h"(h) : "l"(p));
+        w[0] = h;
+      }
+    }
+  }
+  __device__ __forceinline__ void values(float (&l)[V]) const {
+    if constexpr (!VEC) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) l[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if constexpr (DT == RT_F32) l[i] = __uint_as_float(w[i]);
+        else if constexpr (DT == RT_BF16) l[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+        else l[i] = __half2float(__ushort_as_half((unsigned short)(i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xffffu)));
+      }
+    }
+  }
+};
+
+template <int DT, int V, bool VEC>
 __global__ void __launch_bounds__(RT_WARPS * 32) moe_route_kernel(const MoeRouteParams p) {
   using K = RtKey<uint32_t>;
+  constexpr int L = V < 8 ? V : 8, S = V / L;  // sorted lists of a lane
+  constexpr uint32_t PLACE = V - 1;            // the lowest bits of a key: V - 1 - place within the lane
   extern __shared__ unsigned long long rt_smem[];
-  pdl_wait();
-  pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   unsigned long long* keys64 = rt_smem + (size_t)warp * p.E;
   uint32_t* keys32 = reinterpret_cast<uint32_t*>(keys64);
-  const bool by_logits = p.bias == nullptr;                                      // the picks' order
-  const bool groups_by_logits = by_logits && p.group_top == 1;                   // the groups' order
-  const bool need_scores = !by_logits || (p.groups > 1 && !groups_by_logits);
-  const bool need_sum = p.softmax && (need_scores || !p.renormalize);
-  for (long long t = (long long)blockIdx.x * RT_WARPS + warp; t < p.T; t += (long long)gridDim.x * RT_WARPS) {
-    const void* row = static_cast<const char*>(p.logits) + t * p.E * (DT == RT_F32 ? 4 : 2);
+  // candidates, and what is in each place of the order: (expert backwards, value)
+  uint2* list = reinterpret_cast<uint2*>(rt_smem + (size_t)RT_WARPS * p.E + (RT_WARPS * p.E & 1)) + warp * RT_LIST;
+  uint2* place = list + RT_LIST / 2;
+  const int first = lane * V;
+  const bool by_logits = p.bias == nullptr;  // the picks' order
+  const bool need_sum = p.softmax && (!by_logits || !p.renormalize);
+  const bool need_top = p.softmax && (need_sum || (p.groups > 1 && p.group_top == 2));
+  // Groups whose experts are those of 1, 2, 4, .. whole lanes are settled by shuffles, others through shared memory.
+  const int group_lanes = p.group_n % V == 0 ? p.group_n / V : 0;
+  const bool in_lanes = group_lanes > 0 && (group_lanes & (group_lanes - 1)) == 0;
+  const int my_group = in_lanes ? first / p.group_n : 0;
+  const uint32_t below = (1u << lane) - 1u;
+  const uint32_t last_expert = 32 * V - 1, backwards = (uint32_t)(31 - lane) * V;
+  pdl_wait();
+  pdl_launch_dependents();
+  float bias[V];
+  float most_bias = 0.0f;
+  if (!by_logits) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      bias[i] = first + i < p.E ? ld_written(p.bias + first + i) : -INFINITY;
+      if (fabsf(bias[i]) < INFINITY) most_bias = fmaxf(most_bias, fabsf(bias[i]));
+    }
+    most_bias = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most_bias)));
+  }
+  const long long row_bytes = (long long)p.E * (DT == RT_F32 ? 4 : 2);
+  const int step = gridDim.x * RT_WARPS;
+  int t = blockIdx.x * RT_WARPS + warp;
+  const char* row = static_cast<const char*>(p.logits) + t * row_bytes;
+  RtRow<DT, V, VEC> next;
+  if (t < p.T) next.load(row, first, p.E);
+  for (; t < p.T; t += step, row += step * row_bytes) {
     float l[V];
-    float top = -INFINITY;
+    next.values(l);
+    if (t + step < p.T) next.load(row + step * row_bytes, first, p.E);
+    float top = 0.0f, inv_sum = 1.0f;
+    float c[V];
+    if (need_top) {
+      uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = lane + 32 * i;
-      l[i] = e < p.E ? rt_load<DT>(row, e) : -INFINITY;
-      top = rt_max(top, l[i]);
+      for (int i = 0; i < V; ++i) m = max(m, K::of(l[i]));
+      top = K::value(K::warp_max(m));
     }
-    float sum = 1.0f;
-    if (p.softmax) {
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = rt_max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    }
-    uint32_t key[V];
     if (need_sum) {
-      sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < V; ++i) sum += lane + 32 * i < p.E ? expf(l[i] - top) : 0.0f;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    }
-    const float inv_sum = 1.0f / sum;
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = lane + 32 * i;
-      float c = l[i];
-      if (need_scores && e < p.E) {
-        c = p.softmax ? expf(l[i] - top) * inv_sum : 1.0f / (1.0f + expf(-l[i]));
-        if (p.bias != nullptr) c += ld_written(p.bias + e);
-        if (l[i] == -INFINITY) c = -INFINITY;
-      }
-      key[i] = e < p.E ? K::of(c) : 0u;
-    }
-    // fp32 scores are off by less than 2^-20 of the largest score that there can be
-    const float eps = 0x1p-20f * (p.softmax ? inv_sum : 1.0f);
-    bool near = false;
-    if (p.groups > 1) {
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (lane + 32 * i < p.E) keys32[lane + 32 * i] = key[i];
-      __syncwarp();
-      const uint32_t stays = rt_groups<uint32_t>(p, keys32, lane, groups_by_logits ? -1.0f : eps, near);
+      float sum = 0.0f;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const int e = lane + 32 * i;
-        if (by_logits) key[i] = e < p.E ? K::of(l[i]) : 0u;
-        if (e >= p.E || !((stays >> (e / p.group_n)) & 1u)) key[i] = 0u;
+        c[i] = rt_exp_below(l[i], top);
+        sum += c[i];
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      inv_sum = 1.0f / sum;
+    }
+    // Keys.  What is not offered is -inf.
+    uint32_t key[S][L];
+    bool exact = true;  // the place takes no bits from a value
+    if (by_logits) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) c[i] = l[i];
+      if constexpr (DT == RT_F32) {  // (16-bit logits end in zeros)
+        uint32_t lost = 0;
+#pragma unroll
+        for (int i = 0; i < V; ++i) lost |= __float_as_uint(l[i]) & PLACE;
+        exact = !__any_sync(0xffffffffu, lost != 0);
+      }
+    } else {
+      float least = l[0];
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        c[i] = (p.softmax ? c[i] * inv_sum : rt_sigmoid(l[i])) + bias[i];
+        least = fminf(least, l[i]);
+      }
+      if (least == -INFINITY) {
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (l[i] == -INFINITY) c[i] = -INFINITY;
       }
     }
-    int pick = -1;
-    float prev = INFINITY;
-    for (int r = 0; r < (by_logits ? p.k : p.k + 1); ++r) {
-      uint32_t best = 0;
 #pragma unroll
-      for (int i = 0; i < V; ++i) best = max(best, key[i]);
-      const uint32_t m = K::warp_max(best);
-      if (m <= K::NONE) break;
-      if (!by_logits) {
-        const float v = K::value(m);
-        if (r > 0 && prev - v <= 2 * eps + 0x1p-21f * (fabsf(prev) + fabsf(v))) near = true;
-        prev = v;
-      }
-      if (r == p.k) break;
-      int at = 0x7fffffff;
-#pragma unroll
-      for (int i = V - 1; i >= 0; --i)
-        if (key[i] == m) at = lane + 32 * i;
-      const int e = __reduce_min_sync(0xffffffffu, at);
-      if (lane == r) pick = e;
+    for (int i = 0; i < V; ++i) key[i / L][i % L] = (K::of(c[i]) & ~PLACE) | (PLACE - i);
+    // How near two c may come before fp32 cannot tell them apart: each is off by 2^-21 of the largest score that there can be, by its
+    // rounding and by the bits of the place.  (A group's value, without a bias, is not divided by the sum.)
+    const float score = p.softmax && !by_logits ? inv_sum : 1.0f;
+    const float tol = 0x1p-20f * score + (0x1p-22f + V * 0x1p-22f) * (most_bias + score);
+    bool near = false, kept = true;
+    if (p.groups > 1 && !in_lanes) {
+      __syncwarp();
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        if (lane + 32 * i == e) key[i] = 0u;
+        if (first + i < p.E) keys32[first + i] = K::of(c[i]);
+      __syncwarp();
+      const uint32_t stays = rt_groups<uint32_t>(p, keys32, lane, by_logits, top, tol, near);
+      int g = first / p.group_n, at = first - g * p.group_n;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (first + i >= p.E || !((stays >> g) & 1u)) key[i / L][i % L] = 0u;
+        if (++at == p.group_n) { at = 0; ++g; }
+      }
     }
-    if (near) pick = rt_decide_in_64(p, row, DT, keys64, by_logits, top, lane);
-    // weights: lane j has pick j.  Divided by their sum they depend on differences of the logits only, which keeps them
-    // exact where all the picked scores are tiny.
-    const bool there = pick >= 0;
+#pragma unroll
+    for (int s = 0; s < S; ++s) rt_sort<L>(key[s]);
+    if (p.groups > 1 && in_lanes) {
+      // The two largest of the group, by the exact logits where those are what is compared.
+      uint32_t a = 0, b = 0;
+      if (by_logits) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const uint32_t k = K::of(l[i]);
+          b = max(b, min(a, k));
+          a = max(a, k);
+        }
+      } else {
+        a = key[0][0];
+        b = L > 1 ? key[0][1 % L] : 0u;
+#pragma unroll
+        for (int s = 1; s < S; ++s) {
+          b = max(max(b, key[s][1 % L]), min(a, key[s][0]));
+          a = max(a, key[s][0]);
+        }
+      }
+      for (int o = 1; o < group_lanes; o *= 2) {
+        const uint32_t a2 = __shfl_xor_sync(0xffffffffu, a, o), b2 = __shfl_xor_sync(0xffffffffu, b, o);
+        b = max(max(b, b2), min(a, a2));
+        a = max(a, a2);
+      }
+      if (!by_logits) a = a < K::NONE ? a : a & ~PLACE, b = b < K::NONE ? b : b & ~PLACE;
+      const float v = rt_group_value<float>(p, a, b, by_logits, top);
+      const bool inside = first < p.E;
+      const uint32_t mine = inside ? K::of(v) : 0u;
+      int rank = 0;  // groups in front of mine: each of its lanes asks a share of the others
+      for (int j = lane & (group_lanes - 1); j - (lane & (group_lanes - 1)) < p.groups; j += group_lanes) {
+        const uint32_t other = __shfl_sync(0xffffffffu, mine, (j * group_lanes) & 31);
+        rank += j < p.groups && (other > mine || (other == mine && j < my_group)) ? 1 : 0;
+      }
+      for (int o = 1; o < group_lanes; o *= 2) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+      if (!(by_logits && p.group_top == 1)) {
+        const uint32_t last = __ballot_sync(0xffffffffu, inside && rank == p.top_groups - 1);
+        const uint32_t behind = __ballot_sync(0xffffffffu, inside && rank == p.top_groups);
+        const float x = __shfl_sync(0xffffffffu, v, __ffs(last) - 1), y = __shfl_sync(0xffffffffu, v, __ffs(behind) - 1);
+        near = x - y <= 2 * tol;
+      }
+      kept = rank < p.top_groups;
+    }
+    // Candidates: whatever is not below the value that top_k lanes' heads, and one more where it has to be looked at how near it comes,
+    // reach; less what fp32 may be off by, so that fp64 finds among them whatever it may prefer.
+    const bool check = !by_logits || !exact;
+    const int rounds = check ? p.k + 1 : p.k;
+    uint32_t from = 0, rest = 0;
+    if (kept) {
+      rest = key[0][0];
+#pragma unroll
+      for (int s = 1; s < S; ++s) rest = max(rest, key[s][0]);
+      rest &= ~PLACE;
+    }
+#pragma unroll 1
+    for (int r = 0; r < rounds; ++r) {
+      from = K::warp_max(rest);
+      if (rest == from) rest = 0;
+    }
+    if (!by_logits && from > K::NONE) from = K::of(K::value(from) - tol) & ~PLACE;
+    from = max(from, (K::NONE + 1u) & ~PLACE);
+    int n = 0;
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+#pragma unroll
+      for (int d = 0; d < L; ++d) {
+        const bool in = kept && key[s][d] >= from;
+        const uint32_t who = __ballot_sync(0xffffffffu, in);
+        if (who == 0) break;
+        const int at = n + __popc(who & below);
+        if (in && at < 32) list[at] = make_uint2((key[s][d] & PLACE) | backwards, key[s][d] & ~PLACE);
+        n += __popc(who);
+      }
+    }
+    int pick = -1, rank = lane;
+    if (n <= 32 && !near) {
+      // The order of the candidates: value, then expert.
+      if (lane == 0) list[n] = make_uint2(0u, 0u);
+      __syncwarp();
+      const uint2 mine = lane < n ? list[lane] : make_uint2(0u, 0u);
+      const unsigned long long mine64 = ((unsigned long long)mine.y << 32) | mine.x;
+      if (lane < n) {
+        pick = (int)(last_expert - mine.x);
+        rank = 0;
+      }
+      for (int i = 0; i < n; i += 2) {
+        const uint4 two = *reinterpret_cast<const uint4*>(list + i);
+        if (lane < n) rank += ((((unsigned long long)two.y << 32) | two.x) > mine64 ? 1 : 0) + ((((unsigned long long)two.w << 32) | two.z) > mine64 ? 1 : 0);
+      }
+      if (check) {
+        if (rank <= p.k) place[rank] = mine;
+        if (lane == 0) place[32] = make_uint2(0u, 0u);  // (32 candidates at most: nothing is in that place)
+        __syncwarp();
+        bool close = false;
+        if (rank < p.k && pick >= 0) {
+          const uint2 after = place[rank + 1];
+          if (after.y != 0) {
+            close = by_logits ? mine.y == after.y : K::value(mine.y) - K::value(after.y) <= tol;
+            if (close) {  // the same logit and the same bias: a tie, and in the right order
+              const int behind = (int)(last_expert - after.x);
+              if (rt_load<DT>(row, pick) == rt_load<DT>(row, behind) && (by_logits || ld_written(p.bias + pick) == ld_written(p.bias + behind))) close = false;
+            }
+          }
+        }
+        if (__any_sync(0xffffffffu, close)) rank = rt_rank_in_64(p, row, DT, by_logits, pick, n, lane);
+      }
+    } else {
+      // Many equal values, or more picks than heads: a maximum at a time.
+      if (!kept) {
+#pragma unroll
+        for (int s = 0; s < S; ++s)
+#pragma unroll
+          for (int i = 0; i < L; ++i) key[s][i] = 0u;
+      }
+      uint32_t last = 0;
+#pragma unroll 1
+      for (int r = 0; r < rounds && !near; ++r) {
+        uint32_t head = key[0][0];
+#pragma unroll
+        for (int s = 1; s < S; ++s) head = max(head, key[s][0]);
+        const uint32_t value = head & ~PLACE, m = K::warp_max(value);
+        const bool owner = value == m;
+        const uint32_t owners = __ballot_sync(0xffffffffu, owner);
+        if (m <= K::NONE) break;
+        const int first_owner = __ffs(owners) - 1;  // equal values: the lowest lane, and within a lane the lowest place
+        const int e = __shfl_sync(0xffffffffu, first + (int)(PLACE - (head & PLACE)), first_owner);
+        if (check && r > 0 && (by_logits ? m == last : K::value(last) - K::value(m) <= tol)) {
+          const int f = __shfl_sync(0xffffffffu, pick, r - 1);
+          near = !(rt_load<DT>(row, e) == rt_load<DT>(row, f) && (by_logits || ld_written(p.bias + e) == ld_written(p.bias + f)));
+        }
+        last = m;
+        if (r == p.k) break;
+        if (lane == r) pick = e;
+        if (lane == first_owner) {
+#pragma unroll
+          for (int s = 0; s < S; ++s) {
+            if (S == 1 || key[s][0] == head) {
+#pragma unroll
+              for (int i = 0; i + 1 < L; ++i) key[s][i] = key[s][i + 1];
+              key[s][L - 1] = 0u;
+            }
+          }
+        }
+      }
+      if (near) pick = rt_decide_in_64(p, row, DT, keys64, by_logits, lane);
+    }
+    const bool there = rank < p.k && pick >= 0;
     const float lp = there ? rt_load<DT>(row, pick) : -INFINITY;
+    __syncwarp();  // the lists have been read
+    // weights: a lane has the pick of place `rank`.  Divided by their sum they depend on differences of the logits only, which keeps them
+    // exact where all the picked scores are tiny.
     float s;
     if (p.renormalize) {
-      float lm = lp;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) lm = fmaxf(lm, __shfl_xor_sync(0xffffffffu, lm, o));
-      s = p.softmax || lm < -30.0f ? expf(lp - lm) : 1.0f / (1.0f + expf(-lp));
-      if (p.softmax) s += top - top;  // the sum of all scores is NaN where a logit is NaN or +inf
-      if (!there) s = 0.0f;
+      if (p.softmax || __all_sync(0xffffffffu, lp < -30.0f)) {
+        const float most = K::value(K::warp_max(K::of(lp)));  // a NaN among the picks is on top
+        s = there ? expf(lp - most) : 0.0f;
+        if (need_top) s += top - top;  // the sum of all scores is NaN where a logit is NaN or +inf
+      } else {
+        s = there ? __fdividef(1.0f, 1.0f + expf(-lp)) : 0.0f;
+      }
       float all = s;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
-      s = s / all;
+      s = __fdividef(s, all);
     } else {
-      s = p.softmax ? expf(lp - top) * inv_sum : 1.0f / (1.0f + expf(-lp));
+      s = p.softmax ? expf(lp - top) * inv_sum : __fdividef(1.0f, 1.0f + expf(-lp));
     }
-    if (lane < p.k) {
-      p.experts[t * p.k + lane] = pick;
-      p.weights[t * p.k + lane] = there ? s * p.scale : 0.0f;
+    if (rank < p.k) {
+      const long long at = (long long)t * p.k + rank;
+      p.experts[at] = pick;
+      p.weights[at] = there ? s * p.scale : 0.0f;
     }
   }
 }
