@@ -61,18 +61,20 @@ int launch_route(const qg::MoeRouteParams& p, int sms, cudaStream_t s) {
   return vec ? launch_route<DT, true>(p, sms, s) : launch_route<DT, false>(p, sms, s);
 }
 
-// Once per device: the block-table kernel's shared memory and its clusters of more than eight CTAs.
-int ensure_blocks_kernel() {
-  static std::atomic<bool> ready[kMaxDevices];
+// One cluster of `ctas` CTAs.
+template <int WARPS>
+int launch_blocks(const qg::MoeBlocksParams& p, int ctas, cudaStream_t s) {
+  auto kernel = qg::moe_blocks_kernel<WARPS>;
+  static std::atomic<bool> ready[kMaxDevices];  // shared memory and clusters of more than eight are allowed
   int dev = 0;
   CUDA_OK(cudaGetDevice(&dev));
   if (dev < 0 || dev >= kMaxDevices) return fail("device index %d out of range", dev);
-  if (ready[dev].load(std::memory_order_acquire)) return 0;
-  CUDA_OK(cudaFuncSetAttribute(qg::moe_blocks_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               qg::mb_smem_bytes(qg::MB_MAX_THREADS, qg::MB_MAX_E)));
-  CUDA_OK(cudaFuncSetAttribute(qg::moe_blocks_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-  ready[dev].store(true, std::memory_order_release);
-  return 0;
+  if (!ready[dev].load(std::memory_order_acquire)) {
+    CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024));
+    CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    ready[dev].store(true, std::memory_order_release);
+  }
+  return launch_pdl_clusters(kernel, ctas, ctas, WARPS * 32, qg::mb_smem_bytes(WARPS, p.E), s, p);
 }
 
 }  // namespace
@@ -138,7 +140,7 @@ int qgemm_moe_blocks(const int32_t* experts, int32_t* block_metadata, int32_t* r
   if (!aligned(experts, 4) || !aligned(block_metadata, 4) || !aligned(rows, 4) || !aligned(sizes, 4))
     return fail("qgemm_moe_blocks: pointers must be 4-byte aligned");
   int sms = 0;
-  if (ensure_device(&sms) || ensure_blocks_kernel()) return -1;
+  if (ensure_device(&sms)) return -1;
   qg::MoeBlocksParams p;
   p.experts = experts;
   p.meta = block_metadata;
@@ -148,10 +150,16 @@ int qgemm_moe_blocks(const int32_t* experts, int32_t* block_metadata, int32_t* r
   p.E = (int)num_experts;
   p.block_m = (int)block_M;
   p.blocks = (int)qgemm_moe_block_count(entries, num_experts, block_M);
-  const int threads = entries <= 2048 ? 256 : qg::MB_MAX_THREADS;
-  int ctas = 1;
-  while (ctas < qg::MB_MAX_CLUSTER && entries > 4096ll * ctas) ctas *= 2;
-  return launch_pdl_clusters(qg::moe_blocks_kernel, ctas, ctas, threads, qg::mb_smem_bytes(threads, p.E), static_cast<cudaStream_t>(stream), p);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  // us, this form / the general one: 8 picks 1.5 / 3.5, 128 3.2 / 3.6 (256 experts).
+  if (entries > 0 && entries <= qg::MB_FEW)
+    return launch_pdl(qg::moe_blocks_few_kernel, 1, (int)((std::max(entries, num_experts) + 31) / 32 * 32), 0, st, p);
+  // As many warps as keep every pick in a register, from 4096 picks on in clusters: by more CTAs a warp's walk is shorter and the sums over
+  // CTAs longer.  us, CTAs x warps: 2048 picks 1 x 16 4.2, 2 x 16 4.9, 1 x 32 4.7; 8000 8 x 16 5.0, 4 x 16 5.3, 1 x 16 7.3; 16000 8 x 16 5.3,
+  // 16 x 16 5.4; 32768 16 x 16 5.9, 8 x 16 6.1, 16 x 32 6.5; 131072 16 x 32 8.7, 16 x 16 9.7.
+  const bool many = entries > 16 * 512 * qg::MB_ITEMS && qg::mb_smem_bytes(32, p.E) <= 227 * 1024;
+  const int ctas = entries <= 4096 ? 1 : entries <= 24576 ? 8 : qg::MB_MAX_CLUSTER;
+  return many ? launch_blocks<32>(p, ctas, st) : launch_blocks<16>(p, ctas, st);
 }
 
 int qgemm_moe_act_quant(const void* X, const int32_t* rows, int8_t* Y, float* S, int64_t T, int64_t N, int64_t top_k, int x_dtype,
