@@ -20,23 +20,32 @@ bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_
 
 constexpr int kMaxDevices = 64;
 
-template <int TPR, int KEEP, bool BF16>
-int launch_swiglu(const qg::SwigluQuantParams& p, int sms, cudaStream_t s) {
-  auto kernel = qg::swiglu_quant_kernel<TPR, KEEP, BF16>;
-  constexpr int block = qg::sq_block(TPR), rows = block / TPR, smem = qg::sq_smem_bytes(TPR, KEEP);
-  static std::atomic<int> resident[kMaxDevices];  // blocks that an SM holds, once asked
+// A persistent kernel: as many blocks as the SMs hold, or as many as there are rows for.  `resident`: blocks per SM by device, once asked.
+template <typename P>
+int launch_resident(void (*kernel)(P), std::atomic<int>* resident, const P& p, int64_t blocks, int threads, int smem, int sms, cudaStream_t s) {
   int dev = 0, per_sm = 0;
   CUDA_OK(cudaGetDevice(&dev));
   if (dev < 0 || dev >= kMaxDevices) return fail("device index %d out of range", dev);
   if ((per_sm = resident[dev].load(std::memory_order_acquire)) == 0) {
     CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     CUDA_OK(cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
-    CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, block, smem));
-    if (per_sm < 1) return fail("qgemm_swiglu_act_quant: the kernel does not fit on an SM");
+    CUDA_OK(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, smem));
+    if (per_sm < 1) return fail("a kernel of %d threads and %d bytes of shared memory does not fit on an SM", threads, smem);
     resident[dev].store(per_sm, std::memory_order_release);
   }
-  const int64_t grid = std::min<int64_t>((p.M + rows - 1) / rows, (int64_t)per_sm * sms);
-  return launch_pdl(kernel, (int)grid, block, smem, s, p);
+  return launch_pdl(kernel, (int)std::min<int64_t>(blocks, (int64_t)per_sm * sms), threads, smem, s, p);
+}
+template <int TPR, int KEEP, bool BF16>
+int launch_swiglu(const qg::SwigluQuantParams& p, int sms, cudaStream_t s) {
+  static std::atomic<int> resident[kMaxDevices];
+  constexpr int block = qg::sq_block(TPR), rows = block / TPR;
+  return launch_resident(qg::swiglu_quant_kernel<TPR, KEEP, BF16>, resident, p, (p.M + rows - 1) / rows, block, qg::sq_smem_bytes(TPR, KEEP), sms, s);
+}
+template <int TPR, int KEEP, bool BF16>
+int launch_dispatch(const qg::MoeActQuantParams& p, int sms, cudaStream_t s) {
+  static std::atomic<int> resident[kMaxDevices];
+  constexpr int block = qg::mq_block(TPR), rows = block / TPR;
+  return launch_resident(qg::moe_act_quant_kernel<TPR, KEEP, BF16>, resident, p, (p.T + rows - 1) / rows, block, qg::mq_smem_bytes(TPR, KEEP), sms, s);
 }
 
 template <int DT, bool VEC>
@@ -184,17 +193,24 @@ int qgemm_moe_act_quant(const void* X, const int32_t* rows, int8_t* Y, float* S,
   p.T = T;
   p.N = (int)N;
   p.k = (int)top_k;
-  p.is_bf16 = x_dtype == QGEMM_DT_BF16;
   p.round_scale = round_scale != 0;
+  // The fewest threads per row that hold it with eight chunks each: a warp needs no barrier for the row's maximum, and several chunks in
+  // flight per thread do for few rows too.  us, threads x chunks: 16 tokens of 7168 128 x 8 2.8, 256 x 4 2.9, 512 x 2 3.0; 600 of 2048
+  // 32 x 8 3.5, 64 x 4 3.7, 128 x 2 3.4; 4001 of 4096 64 x 8 12.9, 128 x 4 12.7, 256 x 2 15.0; 4096 of 8192 to one place 128 x 8 17.6, 256 x 4 20.9.
   const int64_t chunks = N / 8;
-  int tpr = 32;
-  while (tpr < 256 && chunks > (int64_t)tpr * 4) tpr *= 2;
-  const int64_t rows_per_block = qg::aq_block(tpr) / tpr, grid = (T + rows_per_block - 1) / rows_per_block;
-  auto launch = [&](auto kernel) { return launch_pdl(kernel, (int)grid, qg::aq_block(tpr), 0, static_cast<cudaStream_t>(stream), p); };
-  if (tpr == 32) return launch(qg::moe_act_quant_kernel<32, 4>);
-  if (tpr == 64) return launch(qg::moe_act_quant_kernel<64, 4>);
-  if (tpr == 128) return launch(qg::moe_act_quant_kernel<128, 4>);
-  return launch(qg::moe_act_quant_kernel<256, 4>);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto launch_type = [&](auto bf16) {
+    constexpr bool BF16 = decltype(bf16)::value;
+    if (chunks <= 32) return launch_dispatch<32, 1, BF16>(p, sms, st);
+    if (chunks <= 64) return launch_dispatch<32, 2, BF16>(p, sms, st);
+    if (chunks <= 128) return launch_dispatch<32, 4, BF16>(p, sms, st);
+    if (chunks <= 256) return launch_dispatch<32, 8, BF16>(p, sms, st);
+    if (chunks <= 512) return launch_dispatch<64, 8, BF16>(p, sms, st);
+    if (chunks <= 1024) return launch_dispatch<128, 8, BF16>(p, sms, st);
+    if (chunks <= 2048) return launch_dispatch<256, 8, BF16>(p, sms, st);
+    return launch_dispatch<512, 8, BF16>(p, sms, st);  // above 32768 elements the rest of a row is read a second time
+  };
+  return x_dtype == QGEMM_DT_BF16 ? launch_type(std::true_type{}) : launch_type(std::false_type{});
 }
 
 int qgemm_swiglu_act_quant(const void* X, int8_t* Y, float* S, int64_t M, int64_t F, int x_dtype, int round_scale, void* stream) {

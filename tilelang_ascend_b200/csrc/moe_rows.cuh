@@ -9,6 +9,7 @@
 
 #include "act_quant.cuh"
 #include "common.cuh"
+#include "packed_float.cuh"
 
 namespace qg {
 
@@ -20,70 +21,101 @@ struct MoeActQuantParams {
   long long T;
   int N;            // multiple of 8
   int k;
-  int is_bf16;
   int round_scale;
 };
 
-template <int TPR, int KEEP>
-__global__ void __launch_bounds__(aq_block(TPR)) moe_act_quant_kernel(const MoeActQuantParams p) {
+// aq_quant8 with the fp32 steps in pairs: the same roundings, the same bits.
+template <bool BF16>
+__device__ __forceinline__ uint2 mq_quant8(const uint4& v, f32x2 less_scale, f32x2 rcp) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  const f32x2 magic = f2_make(12582912.0f, 12582912.0f);
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f32x2 x = f2_of_half2<BF16>(w[i]);
+    const f32x2 q0 = f2_mul(x, rcp);
+    const f32x2 q1 = f2_fma(f2_fma(q0, less_scale, x), rcp, q0);
+    const f32x2 q2 = f2_fma(f2_fma(q1, less_scale, x), rcp, q1);
+    f2_get(f2_add(q2, magic), f[2 * i], f[2 * i + 1]);
+  }
+  return make_uint2(aq_pack4(f), aq_pack4(f + 4));
+}
+
+// TPR threads share a row, KEEP chunks of eight elements of it in each one's registers; longer rows are read a second time.  The
+// blocks are persistent: the next row's chunks and places are fetched while this one's codes are stored.
+__host__ __device__ constexpr int mq_block(int tpr) { return tpr == 32 ? 128 : tpr; }
+__host__ __device__ constexpr int mq_smem_bytes(int tpr, int keep) { return keep * 16 * mq_block(tpr); }
+template <int TPR, int KEEP, bool BF16>
+__global__ void __launch_bounds__(mq_block(TPR), KEEP > 4 ? (512 + mq_block(TPR) - 1) / mq_block(TPR) : 1) moe_act_quant_kernel(const MoeActQuantParams p) {
   pdl_wait();
   pdl_launch_dependents();
-  constexpr int ROWS = aq_block(TPR) / TPR;
-  constexpr int WPR = TPR / 32;  // warps per row
-  __shared__ float red[aq_block(TPR) / 32];
-  const int t = threadIdx.x % TPR;
-  const int r = threadIdx.x / TPR;
-  const int warp = threadIdx.x >> 5;
-  const long long row = (long long)blockIdx.x * ROWS + r;
-  const bool live = row < p.T;
+  constexpr int BLOCK = mq_block(TPR), ROWS = BLOCK / TPR, WPR = TPR / 32;
+  static_assert(WPR == 1 || ROWS == 1, "barriers are of the whole block");
+  __shared__ float red[2][WPR];
+  extern __shared__ uint4 mq_slots[];  // a thread's own chunks: no barrier is needed to read them
+  uint4* slot = mq_slots + threadIdx.x;
+  const int t = threadIdx.x % TPR, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int chunks = p.N >> 3;
-  const bool bf16 = p.is_bf16 != 0;
-  const uint4* x = p.X + (live ? row : 0) * chunks;
-
-  uint4 keep[KEEP];
-  uint32_t m2 = 0u;
-  if (live) {
+  const long long R = p.T * p.k;
+  const int step = gridDim.x * ROWS;
+  int row = blockIdx.x * ROWS + threadIdx.x / TPR;
+  int places = -1;  // lane j: place j of the next row (up to 32 of them)
+  auto fetch = [&](int of) {
+    if (of >= p.T) return;
+    const uint4* x = p.X + (long long)of * chunks;
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+      if (t + i * TPR < chunks) cp_async16(smem_u32(slot + i * BLOCK), x + t + i * TPR);
+    if (lane < p.k) places = ld_written(p.rows + (long long)of * p.k + lane);
+  };
+  fetch(row);
+  for (int turn = 0; row < p.T; row += step, turn ^= 1) {
+    const uint4* x = p.X + (long long)row * chunks;
+    uint4 keep[KEEP];
+    uint32_t m2 = 0u;
+    cp_async_wait();
 #pragma unroll
     for (int i = 0; i < KEEP; ++i) {
-      const int c = t + i * TPR;
-      if (c < chunks) {
-        keep[i] = ld_written(x + c);
-        m2 = aq_absmax8(keep[i], bf16, m2);
+      if (t + i * TPR < chunks) {
+        keep[i] = slot[i * BLOCK];
+        m2 = aq_absmax8(keep[i], BF16, m2);
       }
     }
-    for (int c = t + KEEP * TPR; c < chunks; c += TPR) m2 = aq_absmax8(ld_written(x + c), bf16, m2);
-  }
-  float m = aq_pair_max(m2, bf16);
+    for (int c = t + KEEP * TPR; c < chunks; c += TPR) m2 = aq_absmax8(ld_written(x + c), BF16, m2);
+    float m = aq_pair_max(m2, BF16);
+    m = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(m)));
+    const int at_lane = places;
+    fetch(row + step);  // every slot has been read
+    if (WPR > 1) {
+      if (lane == 0) red[turn][warp] = m;
+      __syncthreads();
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  if (WPR > 1) {
-    if ((threadIdx.x & 31) == 0) red[warp] = m;
-    __syncthreads();
+      for (int w = 0; w < WPR; ++w) m = fmaxf(m, red[turn][w]);
+    }
+    const float amax = fmaxf(m, 1e-4f);
+    float scale = __fdiv_rn(amax, 127.0f);
+    if (p.round_scale) scale = aq_pow2_ceil(scale);
+    const float rcp = __frcp_rn(scale);
+    const f32x2 less_scale = f2_make(-scale, -scale), rcp2 = f2_make(rcp, rcp);
+    uint2 code[KEEP];
 #pragma unroll
-    for (int w = 0; w < WPR; ++w) m = fmaxf(m, red[r * WPR + w]);
-  }
-  if (!live) return;
-
-  const float amax = fmaxf(m, 1e-4f);
-  float scale = __fdiv_rn(amax, 127.0f);
-  if (p.round_scale) scale = aq_pow2_ceil(scale);
-  const float rcp = __frcp_rn(scale);
-  const long long R = p.T * p.k;
-  auto store = [&](int c, const uint2& v) {
+    for (int i = 0; i < KEEP; ++i) code[i] = mq_quant8<BF16>(keep[i], less_scale, rcp2);
     for (int j = 0; j < p.k; ++j) {
-      const int at = ld_written(p.rows + row * p.k + j);
+      const int at = j < 32 ? __shfl_sync(0xffffffffu, at_lane, j) : ld_written(p.rows + (long long)row * p.k + j);
       const long long to = at >= 0 ? at : -2ll - at;
       if (to < 0 || to >= R) continue;
-      reinterpret_cast<uint2*>(p.Y)[to * chunks + c] = at >= 0 ? v : make_uint2(0u, 0u);
-      if (c == 0) p.S[to] = at >= 0 ? scale : 0.0f;
-    }
-  };
+      uint2* y = reinterpret_cast<uint2*>(p.Y) + to * chunks;
+      const uint32_t mask = at >= 0 ? 0xffffffffu : 0u;
 #pragma unroll
-  for (int i = 0; i < KEEP; ++i) {
-    const int c = t + i * TPR;
-    if (c < chunks) store(c, aq_quant8(keep[i], bf16, scale, rcp));
+      for (int i = 0; i < KEEP; ++i)
+        if (t + i * TPR < chunks) __stcs(y + t + i * TPR, make_uint2(code[i].x & mask, code[i].y & mask));
+      for (int c = t + KEEP * TPR; c < chunks; c += TPR) {
+        const uint2 v = mq_quant8<BF16>(ld_written(x + c), less_scale, rcp2);
+        __stcs(y + c, make_uint2(v.x & mask, v.y & mask));
+      }
+      if (t == 0) p.S[to] = at >= 0 ? scale : 0.0f;
+    }
   }
-  for (int c = t + KEEP * TPR; c < chunks; c += TPR) store(c, aq_quant8(ld_written(x + c), bf16, scale, rcp));
 }
 
 struct MoeCombineParams {

@@ -17,6 +17,7 @@
 
 #include "act_quant.cuh"
 #include "common.cuh"
+#include "packed_float.cuh"
 
 namespace qg {
 
@@ -28,42 +29,6 @@ struct SwigluQuantParams {
   int F;            // multiple of 8
   int round_scale;
 };
-
-// ------------------------------------------------------------------------ two fp32 values in a 64-bit register
-using f32x2 = unsigned long long;
-__device__ __forceinline__ f32x2 f2_make(float lo, float hi) {
-  f32x2 v;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi));
-  return v;
-}
-__device__ __forceinline__ void f2_get(f32x2 v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-__device__ __forceinline__ f32x2 f2_mul(f32x2 a, f32x2 b) {
-  f32x2 v;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
-  return v;
-}
-__device__ __forceinline__ f32x2 f2_add(f32x2 a, f32x2 b) {
-  f32x2 v;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
-  return v;
-}
-__device__ __forceinline__ f32x2 f2_fma(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 v;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
-  return v;
-}
-// The largest of three absolute values; NaN if one is.
-__device__ __forceinline__ float f3_max_abs(float a, float b, float c) {
-  float v;
-  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
-  return v;
-}
-template <bool BF16>
-__device__ __forceinline__ f32x2 f2_of_half2(uint32_t w) {
-  if constexpr (BF16) return f2_make(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
-  return f2_make(f.x, f.y);
-}
 
 // --------------------------------------------------------------------------------------------------- a in fp32 and fp64
 __device__ __forceinline__ float sq_exp2(float t) {
