@@ -575,3 +575,34 @@ def test_function_transforms_are_refused():
                  lambda t: q.moe_combine(t, rows, torch.zeros((4, 2), device="cuda"))):
         with pytest.raises(RuntimeError):
             torch.vmap(call)(x)
+
+
+# 148 SMs: tiles of 128 columns in one round, of 256 in several rounds with a cut last one, of 256 in one round
+@pytest.mark.parametrize("sizes,K,N", [((5, 0, 300, 1, 0, 0, 129, 2), 272, 528), ((700, 0, 1, 900, 128, 0, 640, 300, 0, 1100), 144, 2064),
+                                       ((0, 0, 0, 0, 257), 1040, 256), ((64,) * 40, 512, 4096)])
+@pytest.mark.parametrize("layout", ["KN", "NK"])
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_grouped_product_passes_over_entries_without_rows(sizes, K, N, layout, dt):
+    """Entries without rows behind the others, in front of them and between them change nothing: results, accumulators, rows that no
+    block covers, and the calls behind."""
+    g = torch.Generator(device="cuda").manual_seed(K + N)
+    G, R = len(sizes), sum(sizes)
+    A = torch.randint(-128, 128, (R + 9, K), dtype=torch.int8, generator=g, device="cuda")
+    B = torch.randint(-128, 128, (G, K, N) if layout == "KN" else (G, N, K), dtype=torch.int8, generator=g, device="cuda")
+    s, sa = torch.rand((G, N), generator=g, device="cuda"), torch.rand(R + 9, generator=g, device="cuda")
+    used = q.build_block_metadata(sizes, 128)
+    none = torch.tensor([[-1, R, 0], [0, 0, 0], [G, 0, 5], [0, R + 9, 5], [1, 3, -7]], dtype=torch.int32)
+    most = G + (R + 9) // 128
+    tables = [torch.cat([used, none[:1].repeat(most, 1)]), torch.cat([none.repeat(most, 1), used]),
+              torch.cat([torch.cat([none, u[None]]) for u in used] + [none[:1].repeat(most, 1)])]
+    kw = dict(out_dtype=dt, b_layout=layout)
+    want, acc = q.grouped_quant_matmul(A, B, used.cuda(), s, sa, return_accumulators=True, **kw)
+    for table in tables:
+        got, got_acc = q.grouped_quant_matmul(A, B, table.cuda(), s, sa, return_accumulators=True, **kw)
+        assert torch.equal(got, want) and torch.equal(got_acc, acc)
+        assert torch.equal(q.grouped_quant_matmul(A, B, table.cuda(), s, sa, **kw), want)
+        out = torch.full_like(want, 3.0)
+        q.grouped_quant_matmul(A, B, table.cuda(), s, sa, out=out, **kw)
+        assert torch.equal(out[:R], want[:R]) and (out[R:] == 3.0).all()
+    empty = q.grouped_quant_matmul(A, B, none.repeat(most, 1).cuda(), s, sa, **kw)
+    assert (empty == 0).all()

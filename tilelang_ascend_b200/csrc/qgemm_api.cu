@@ -76,6 +76,10 @@ int set_smem_w8() {
   if (set_smem(qg::w8a8_gemm_kernel<BN, false, true>, C::SMEM_BYTES)) return -1;
   if (set_smem(qg::w8a8_gemm_kernel<BN, true, false>, C::SMEM_BYTES)) return -1;
   if (set_smem(qg::w8a8_gemm_kernel<BN, true, true>, C::SMEM_BYTES)) return -1;
+  if (set_smem(qg::w8a8_gemm_kernel<BN, false, false, qg::W8_ALONE, true>, C::SMEM_BYTES)) return -1;
+  if (set_smem(qg::w8a8_gemm_kernel<BN, false, true, qg::W8_ALONE, true>, C::SMEM_BYTES)) return -1;
+  if (set_smem(qg::w8a8_gemm_kernel<BN, true, false, qg::W8_ALONE, true>, C::SMEM_BYTES)) return -1;
+  if (set_smem(qg::w8a8_gemm_kernel<BN, true, true, qg::W8_ALONE, true>, C::SMEM_BYTES)) return -1;
   if constexpr (BN == 256) {  // the forms of two CTAs
     if (set_smem(qg::w8a8_gemm_kernel<256, false, false, qg::W8_SPLITK>, C::SMEM_BYTES)) return -1;
     if (set_smem(qg::w8a8_gemm_kernel<256, false, true, qg::W8_SPLITK>, C::SMEM_BYTES)) return -1;
@@ -230,8 +234,9 @@ int w8_group_m(int64_t m_tiles, int64_t k_bytes, int64_t groups, int64_t b_bytes
 
 template <int BN, bool NK, bool BF>
 int launch_w8(const CUtensorMap& tmA, const CUtensorMap& tmB, const CUtensorMap& tmC, const qg::W8A8Params& p, int grid,
-              cudaStream_t s) {
-  return launch_pdl(qg::w8a8_gemm_kernel<BN, NK, BF>, grid, qg::W8_THREADS, qg::W8Cfg<BN>::SMEM_BYTES, s, tmA, tmB, tmC, p);
+              cudaStream_t s, bool skip) {
+  auto kernel = skip ? qg::w8a8_gemm_kernel<BN, NK, BF, qg::W8_ALONE, true> : qg::w8a8_gemm_kernel<BN, NK, BF>;
+  return launch_pdl(kernel, grid, qg::W8_THREADS, qg::W8Cfg<BN>::SMEM_BYTES, s, tmA, tmB, tmC, p);
 }
 
 // The forms in which a cluster of two CTAs makes a tile: `clusters` of them.
@@ -807,12 +812,14 @@ static int w8a8_impl(const int8_t* A, const int8_t* B, const float* scale_b, con
     if (nk) return bf ? launch_w8_clusters<true, true, form>(tmA, tmB, tmC, p, grid, s) : launch_w8_clusters<true, false, form>(tmA, tmB, tmC, p, grid, s);
     return bf ? launch_w8_clusters<false, true, form>(tmA, tmB, tmC, p, grid, s) : launch_w8_clusters<false, false, form>(tmA, tmB, tmC, p, grid, s);
   }
+  // A table with as many entries as its rows can need at most: from qgemm_moe_blocks, and probably not all in use.
+  const bool skip = meta != nullptr && num_blocks >= qgemm_moe_block_count(M, batch, qg::W8_BM);
   if (BN == 256) {
-    if (nk) return bf ? launch_w8<256, true, true>(tmA, tmB, tmC, p, grid, s) : launch_w8<256, true, false>(tmA, tmB, tmC, p, grid, s);
-    return bf ? launch_w8<256, false, true>(tmA, tmB, tmC, p, grid, s) : launch_w8<256, false, false>(tmA, tmB, tmC, p, grid, s);
+    if (nk) return bf ? launch_w8<256, true, true>(tmA, tmB, tmC, p, grid, s, skip) : launch_w8<256, true, false>(tmA, tmB, tmC, p, grid, s, skip);
+    return bf ? launch_w8<256, false, true>(tmA, tmB, tmC, p, grid, s, skip) : launch_w8<256, false, false>(tmA, tmB, tmC, p, grid, s, skip);
   }
-  if (nk) return bf ? launch_w8<128, true, true>(tmA, tmB, tmC, p, grid, s) : launch_w8<128, true, false>(tmA, tmB, tmC, p, grid, s);
-  return bf ? launch_w8<128, false, true>(tmA, tmB, tmC, p, grid, s) : launch_w8<128, false, false>(tmA, tmB, tmC, p, grid, s);
+  if (nk) return bf ? launch_w8<128, true, true>(tmA, tmB, tmC, p, grid, s, skip) : launch_w8<128, true, false>(tmA, tmB, tmC, p, grid, s, skip);
+  return bf ? launch_w8<128, false, true>(tmA, tmB, tmC, p, grid, s, skip) : launch_w8<128, false, false>(tmA, tmB, tmC, p, grid, s, skip);
 }
 
 int qgemm_w8a8(const int8_t* A, const int8_t* B, const float* scale_b, const float* scale_a, void* C,

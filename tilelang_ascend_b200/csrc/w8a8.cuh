@@ -177,7 +177,12 @@ __device__ __forceinline__ void w8_zero_uncovered(const W8A8Params& p, int warp4
 // hand an accumulator back to it.  Traffic is what bounds these shapes, for what it costs in time and, at the power limit, in
 // clock: 4096 x 4096 x 14336 166 -> 148 us (3.2 POPS, cuBLASLt's plain int8 GEMM 3.0; tensor pipe 92 % of active cycles instead of
 // 79, 1.9 GB from L2 into the SMs instead of 2.8), 16 x 512 x 7168 x 2048 [N, K] 101 -> 89.  Which shapes take it: w8_pair_pays in qgemm_api.cu.
-template <int BN, bool B_NK, bool OUT_BF16, W8Form FORM = W8_ALONE>
+//
+// SKIP: for tables with entries that have no rows (one that was made on the device has as many entries as its picks could need): all three
+// roles pass over their items.  us, without / with it: 16 tokens to 4 of 64 experts, 7168 x 4096, 44 of 64 entries in use 229 / 198; 4096
+// tokens, 4096 x 2048, 158 of 191 184 / 150.  A form of its own, because the look-up in the MMA warp costs 1 - 3 % of a call
+// whose table has none, 14 % of 1500 rows in 12 groups, 4096 x 1024.
+template <int BN, bool B_NK, bool OUT_BF16, W8Form FORM = W8_ALONE, bool SKIP = false>
 __global__ void __launch_bounds__(W8_THREADS, 1)
 w8a8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                  const __grid_constant__ CUtensorMap tmC, const W8A8Params p) {
@@ -185,6 +190,7 @@ w8a8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   constexpr int STAGES = Cfg::STAGES;
   constexpr bool SPLITK = FORM == W8_SPLITK, PAIR = FORM == W8_PAIR;
   static_assert(!(SPLITK && B_NK), "K is cut for weights [K, N] only");
+  static_assert(!SKIP || FORM == W8_ALONE, "row tables are for tiles of one CTA");
   // Two warps share the columns of 32 rows and store them in pieces of 64: an item of 128 columns at least (a half-width one, or
   // a CTA's half of a tile whose K is cut, comes from 256).
   static_assert(BN == 128 || (BN == 256 && (BN / 2) % 128 == 0), "columns of a tile");
@@ -267,6 +273,7 @@ w8a8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       const bool idle = PAIR && p.withhold == 3 + crank && tile_first == tile_stride - 1;  // test hook: this CTA copies nothing
       for (int tile = idle ? p.num_items : tile_first; ok && tile < p.num_items; tile += tile_stride) {
         const W8Tile t = w8_tile<PAIR>(p, tile, crank);
+        if (SKIP && t.rows <= 0) continue;
         const int m0 = t.m0, n0 = t.n0;
         const int b_boxes = B_NK ? 1 : (t.bn + 127) / 128;  // 128-column boxes of B actually needed
         const uint32_t tx = Cfg::A_BYTES + (B_NK ? (uint32_t)Cfg::B_BYTES : (uint32_t)(b_boxes * W8_BK * 128));
@@ -330,11 +337,22 @@ w8a8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     uint32_t phase = 0;
     int it = 0;
     bool ok = true;
-    for (int tile = PAIR && crank != 0 ? p.num_items : tile_first; ok && tile < p.num_items; tile += tile_stride, ++it) {
+    auto empty_item = [&](int item) {  // (the vote tells the compiler that the warp stays together)
+      return SKIP && item < p.num_items && __any_sync(0xffffffffu, w8_tile<PAIR>(p, item, crank).rows <= 0);
+    };
+    bool nothing_next = empty_item(tile_first);  // there is nothing to do for the next item
+    for (int tile = PAIR && crank != 0 ? p.num_items : tile_first; ok && tile < p.num_items; tile += tile_stride) {
+      if (nothing_next) {
+        nothing_next = empty_item(tile + tile_stride);
+        continue;
+      }
+      // Whether the next item is empty is looked up behind a few k blocks' MMAs, which keep the tensor core busy meanwhile.
+      const int look_up = min(kb_begin + 2, kb_end - 1);
       const uint32_t bn = (uint32_t)((tile < p.split_from) ? p.bn : (p.bn >> 1));
       const uint32_t idesc = make_idesc(ACC_S32, FMT_S8, FMT_S8, 0, B_NK ? 0 : 1, PAIR ? 2 * W8_BM : W8_BM, bn);
       const int buf = it & 1;
       const uint32_t tphase = (it >> 1) & 1;
+      ++it;
       if (!mbar_wait_warp(&tempty[buf], tphase ^ 1u, ctl, ST_TIMEOUT_MMA)) { ok = false; break; }
       tc_fence_after_sync();
       const uint32_t d = tmem_base + buf * BN;
@@ -354,6 +372,7 @@ w8a8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           if constexpr (PAIR) umma_commit_pair(&empty[stage]);
           else umma_commit(&empty[stage]);
         }
+        if (SKIP && kb == look_up) nothing_next = empty_item(tile + tile_stride);
         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
       }
       if (ok && elect_one_sync()) {  // the elected lane is the same one every time
@@ -395,10 +414,12 @@ w8a8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     // (row, four columns): piece (col / 4, row) at ((col / 4) * 128 + row) * 16, so that a warp's 32 rows are
     // 512 contiguous bytes for the sender's stores and the receiver's loads alike
     const uint32_t part_row = smem_u32(smem) + (uint32_t)(q * 32 + lane) * 16u;
-    for (int tile = tile_first; tile < p.num_items; tile += tile_stride, ++it) {
+    for (int tile = tile_first; tile < p.num_items; tile += tile_stride) {
       const W8Tile t = w8_tile<PAIR>(p, tile, crank);
+      if (SKIP && t.rows <= 0) continue;
       const int buf = it & 1;
       const uint32_t tphase = (it >> 1) & 1;
+      ++it;
       const int m = t.m0 + q * 32 + lane;
       const bool row_ok = q * 32 + lane < t.rows;
       float sa = 1.0f;
