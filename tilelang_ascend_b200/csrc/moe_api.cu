@@ -48,17 +48,22 @@ int launch_dispatch(const qg::MoeActQuantParams& p, int sms, cudaStream_t s) {
   return launch_resident(qg::moe_act_quant_kernel<TPR, KEEP, BF16>, resident, p, (p.T + rows - 1) / rows, block, qg::mq_smem_bytes(TPR, KEEP), sms, s);
 }
 
+template <int DT, int V, bool VEC>
+int launch_route(const qg::MoeRouteParams& p, int sms, cudaStream_t s) {
+  // More blocks than the SMs hold, so that one that has a token to decide in fp64 is not waited for with its others; but what a warp does
+  // once is worth 50 instructions a token.  us, 8 / 12 / 24 blocks per SM: 16384 x 256 22.0 / 21.7 / 21.8, 16384 x 64 9.4 / 8.5 / 9.8, 16384 x
+  // 128 15.2 / 13.8 / 14.9, 9000 x 384 16.5 / 18.1 / 19.5; as many as they hold (7) 23.7 for the first.
+  const int64_t blocks = std::min<int64_t>((p.T + qg::RT_WARPS - 1) / qg::RT_WARPS, (V <= 8 ? 12ll : 8ll) * sms);
+  return launch_pdl(qg::moe_route_kernel<DT, V, VEC>, (int)blocks, qg::RT_WARPS * 32, qg::rt_smem_bytes(p.E), s, p);
+}
 template <int DT, bool VEC>
 int launch_route(const qg::MoeRouteParams& p, int sms, cudaStream_t s) {
-  const long long blocks = std::min<long long>((p.T + qg::RT_WARPS - 1) / qg::RT_WARPS, 8ll * sms);
-  const int smem = qg::rt_smem_bytes(p.E);
-  auto launch = [&](auto kernel) { return launch_pdl(kernel, (int)blocks, qg::RT_WARPS * 32, smem, s, p); };
-  if (p.E <= 32) return launch(qg::moe_route_kernel<DT, 1, VEC>);
-  if (p.E <= 64) return launch(qg::moe_route_kernel<DT, 2, VEC>);
-  if (p.E <= 128) return launch(qg::moe_route_kernel<DT, 4, VEC>);
-  if (p.E <= 256) return launch(qg::moe_route_kernel<DT, 8, VEC>);
-  if (p.E <= 512) return launch(qg::moe_route_kernel<DT, 16, VEC>);
-  return launch(qg::moe_route_kernel<DT, 32, VEC>);
+  if (p.E <= 32) return launch_route<DT, 1, VEC>(p, sms, s);
+  if (p.E <= 64) return launch_route<DT, 2, VEC>(p, sms, s);
+  if (p.E <= 128) return launch_route<DT, 4, VEC>(p, sms, s);
+  if (p.E <= 256) return launch_route<DT, 8, VEC>(p, sms, s);
+  if (p.E <= 512) return launch_route<DT, 16, VEC>(p, sms, s);
+  return launch_route<DT, 32, VEC>(p, sms, s);
 }
 template <int DT>
 int launch_route(const qg::MoeRouteParams& p, int sms, cudaStream_t s) {

@@ -11,9 +11,11 @@
 // scores: one token in some hundreds).
 //
 // One warp per token.  A lane has V consecutive experts as 32-bit keys in the order of the values, whose lowest bits are the place within
-// the lane, and sorts them (in lists of eight) in registers.  A pick is then a maximum over the lanes' heads, one redux instruction, and a
-// step of the winning lane's list: 14 instructions where a search of all values for the maximum would be 40.  E 4 bytes of
-// reading per token are 300 - 400 instructions of a warp, which is what bounds it: 16384 x 256 is 1.5 us of memory and 5 of issue.
+// the lane, and sorts them (in lists of eight) in registers.  The value that top_k lanes' heads reach bounds the picks from below: a
+// maximum over the heads, one redux instruction, top_k times.  The keys from there on, a dozen or so, are gathered by votes
+// and each lane counts how many come before its own.  (A maximum over the heads per pick, with a step of the winner's list, was 32
+// instructions a pick; this is 130 for all.)  What bounds it is issue: 16384 x 256 in bf16 with bias and groups is 1.5 us of memory and 750
+// instructions of a warp per token, 11 us at one a cycle; measured 21.7.
 #pragma once
 
 #include "common.cuh"
@@ -58,7 +60,7 @@ __device__ __forceinline__ float rt_max(float a, float b) {
 }
 
 // Values as unsigned numbers of the same order; NaN above everything, both zeros alike, -inf (not offered) at RT_NONE.
-constexpr int RT_LIST = 68;  // two lists of 34 entries of a warp, on a 16-byte boundary
+constexpr int RT_LIST = 72;  // two lists of 36 entries of a warp, on a 16-byte boundary
 __host__ __device__ constexpr int rt_smem_bytes(int E) { return 8 * (RT_WARPS * E + (RT_WARPS * E & 1) + RT_WARPS * RT_LIST); }
 
 template <typename K> struct RtKey;
@@ -317,8 +319,10 @@ struct RtRow {
   }
 };
 
+// Blocks per SM that the registers have to allow.  us, 16384 x 256 with groups: 108 registers 30, 80 25.6, 72 23.7, 64 25.5, 48 27.0.
+__host__ __device__ constexpr int rt_min_blocks(int V) { return V <= 8 ? 7 : V == 16 ? 4 : 2; }
 template <int DT, int V, bool VEC>
-__global__ void __launch_bounds__(RT_WARPS * 32) moe_route_kernel(const MoeRouteParams p) {
+__global__ void __launch_bounds__(RT_WARPS * 32, rt_min_blocks(V)) moe_route_kernel(const MoeRouteParams p) {
   using K = RtKey<uint32_t>;
   constexpr int L = V < 8 ? V : 8, S = V / L;  // sorted lists of a lane
   constexpr uint32_t PLACE = V - 1;            // the lowest bits of a key: V - 1 - place within the lane
@@ -482,9 +486,12 @@ __global__ void __launch_bounds__(RT_WARPS * 32) moe_route_kernel(const MoeRoute
       rest &= ~PLACE;
     }
 #pragma unroll 1
-    for (int r = 0; r < rounds; ++r) {
-      from = K::warp_max(rest);
-      if (rest == from) rest = 0;
+    for (int r = 0; r < rounds; r += 3) {  // (one or two too many make candidates more, no fewer)
+#pragma unroll
+      for (int j = 0; j < 3; ++j) {
+        from = K::warp_max(rest);
+        if (rest == from) rest = 0;
+      }
     }
     if (!by_logits && from > K::NONE) from = K::of(K::value(from) - tol) & ~PLACE;
     from = max(from, (K::NONE + 1u) & ~PLACE);
@@ -504,17 +511,21 @@ __global__ void __launch_bounds__(RT_WARPS * 32) moe_route_kernel(const MoeRoute
     int pick = -1, rank = lane;
     if (n <= 32 && !near) {
       // The order of the candidates: value, then expert.
-      if (lane == 0) list[n] = make_uint2(0u, 0u);
+      if (lane < 4) list[n + lane] = make_uint2(0u, 0u);
       __syncwarp();
       const uint2 mine = lane < n ? list[lane] : make_uint2(0u, 0u);
       const unsigned long long mine64 = ((unsigned long long)mine.y << 32) | mine.x;
+      int in_front = 0;
+      for (int i = 0; i < n; i += 4) {
+        const uint4 two = *reinterpret_cast<const uint4*>(list + i), more = *reinterpret_cast<const uint4*>(list + i + 2);
+        in_front += (((unsigned long long)two.y << 32) | two.x) > mine64;
+        in_front += (((unsigned long long)two.w << 32) | two.z) > mine64;
+        in_front += (((unsigned long long)more.y << 32) | more.x) > mine64;
+        in_front += (((unsigned long long)more.w << 32) | more.z) > mine64;
+      }
       if (lane < n) {
         pick = (int)(last_expert - mine.x);
-        rank = 0;
-      }
-      for (int i = 0; i < n; i += 2) {
-        const uint4 two = *reinterpret_cast<const uint4*>(list + i);
-        if (lane < n) rank += ((((unsigned long long)two.y << 32) | two.x) > mine64 ? 1 : 0) + ((((unsigned long long)two.w << 32) | two.z) > mine64 ? 1 : 0);
+        rank = in_front;
       }
       if (check) {
         if (rank <= p.k) place[rank] = mine;
