@@ -316,8 +316,11 @@ int qgemm_moe_combine(const void* Y, const int32_t* rows, const float* weights, 
   const int64_t grid = T * p.parts;
   if (grid > 0x7fffffffll) return fail("qgemm_moe_combine: too many tokens (%lld of %lld)", (long long)T, (long long)N);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == QGEMM_DT_BF16 ? launch_pdl(qg::moe_combine_kernel<true>, (int)grid, qg::MC_THREADS, 0, s, p)
-                                : launch_pdl(qg::moe_combine_kernel<false>, (int)grid, qg::MC_THREADS, 0, s, p);
+  auto launch = [&](auto kernel) { return launch_pdl(kernel, (int)grid, qg::MC_THREADS, 0, s, p); };
+  const bool bf16 = dtype == QGEMM_DT_BF16;
+  if (top_k <= 2) return bf16 ? launch(qg::moe_combine_kernel<true, 2>) : launch(qg::moe_combine_kernel<false, 2>);
+  if (top_k <= 4) return bf16 ? launch(qg::moe_combine_kernel<true, 4>) : launch(qg::moe_combine_kernel<false, 4>);
+  return bf16 ? launch(qg::moe_combine_kernel<true, 8>) : launch(qg::moe_combine_kernel<false, 8>);
 }
 
 }  // extern "C"

@@ -4,7 +4,8 @@
 // places of its token.  A row is read once, 2 N bytes, and written top_k times, N bytes each.
 //
 // moe_combine_kernel: out[t] = cast(base[t] + sum_j weights[t, j] * y[rows[t, j]]), fp32, j in order.  A thread has 16 bytes of a row.
-// 2 top_k N bytes in and 2 N out per token.
+// 2 top_k N bytes in and 2 N out per token, which is what bounds it once up to eight entries are in flight per thread: 4096 tokens of 7168, eight
+// entries each, 6.7 TB/s (79 us; 92 with one entry after another, and 16 tokens 1.8 us instead of 3.0).
 #pragma once
 
 #include "act_quant.cuh"
@@ -130,26 +131,41 @@ struct MoeCombineParams {
   int parts;             // blocks per token
 };
 
-constexpr int MC_THREADS = 256;
+constexpr int MC_THREADS = 128;  // (256: 4096 tokens of 7168, eight entries each 81.5 us instead of 79.1)
 
-template <bool BF16>
+// AHEAD entries of a token are in flight at a time: their places and weights, then their 16 bytes.
+template <bool BF16, int AHEAD>
 __global__ void __launch_bounds__(MC_THREADS) moe_combine_kernel(const MoeCombineParams p) {
   pdl_wait();
   pdl_launch_dependents();
   const long long t = blockIdx.x / p.parts;
   const int chunks = p.N >> 3, c = (int)(blockIdx.x - t * p.parts) * MC_THREADS + threadIdx.x;
   if (c >= chunks) return;
-  float acc[8], v[8];
+  float acc[8], f[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) acc[i] = 0.0f;
   if (p.base != nullptr) aq_unpack8(ld_written(p.base + t * chunks + c), BF16, acc);
-  for (int j = 0; j < p.k; ++j) {
-    const int row = ld_written(p.rows + t * p.k + j);
-    if (row < 0 || row >= p.R) continue;
-    const float w = ld_written(p.weights + t * p.k + j);
-    aq_unpack8(ld_written(p.Y + (long long)row * chunks + c), BF16, v);
+  const int* rows = p.rows + t * p.k;
+  const float* weights = p.weights + t * p.k;
+  for (int j0 = 0; j0 < p.k; j0 += AHEAD) {
+    int row[AHEAD];
+    float w[AHEAD];
+    uint4 v[AHEAD];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] = fmaf(w, v[i], acc[i]);
+    for (int j = 0; j < AHEAD; ++j) {
+      row[j] = j0 + j < p.k ? ld_written(rows + j0 + j) : -1;
+      w[j] = j0 + j < p.k ? ld_written(weights + j0 + j) : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j)
+      if (row[j] >= 0 && row[j] < p.R) v[j] = ld_written(p.Y + (long long)row[j] * chunks + c);
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) {
+      if (row[j] < 0 || row[j] >= p.R) continue;
+      aq_unpack8(v[j], BF16, f);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] = fmaf(w[j], f[i], acc[i]);
+    }
   }
   p.out[t * chunks + c] = make_uint4(pack_out2<BF16>(acc[0], acc[1]), pack_out2<BF16>(acc[2], acc[3]), pack_out2<BF16>(acc[4], acc[5]),
                                      pack_out2<BF16>(acc[6], acc[7]));
