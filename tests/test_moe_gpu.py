@@ -606,3 +606,90 @@ def test_grouped_product_passes_over_entries_without_rows(sizes, K, N, layout, d
         assert torch.equal(out[:R], want[:R]) and (out[R:] == 3.0).all()
     empty = q.grouped_quant_matmul(A, B, none.repeat(most, 1).cuda(), s, sa, **kw)
     assert (empty == 0).all()
+
+
+# ------------------------------------------------------------------------------------------- forms and their edges
+# one, two, .. eight chunks per thread; rows shared by 32 .. 512 threads, full and one chunk over; few rows and more than the blocks
+# that the SMs hold; rows that do not fit a thread's registers
+GATE_FORMS = [(20000, 8), (20000, 256), (9000, 264), (7000, 512), (6000, 776), (5000, 1024), (5000, 1288), (5000, 1536), (4000, 1792),
+              (4000, 2048), (3000, 2056), (2500, 3584), (2500, 4096), (1500, 4104), (1300, 7168), (1300, 8192), (700, 8200), (700, 14336), (400, 16392),
+              (300, 28672), (200, 32776), (260, 256), (259, 2048), (258, 2056), (130, 4104), (65, 8200), (64, 16392)]
+
+
+@pytest.mark.parametrize("M,F", GATE_FORMS)
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_gate_forms(M, F, dt):
+    g = torch.Generator(device="cuda").manual_seed(M + F)
+    x = (torch.randn((M, 2 * F), generator=g, device="cuda") * (0.5 + 3 * torch.rand((M, 1), generator=g, device="cuda"))).to(dt)
+    for round_scale in (False, True):
+        y, s = q.swiglu_act_quant(x, round_scale)
+        y_ref, s_ref = mo.swiglu_act_quant_ref(x, round_scale)
+        assert torch.equal(s, s_ref) and torch.equal(y, y_ref)
+
+
+@pytest.mark.parametrize("T,N,k", [(9000, 8, 3), (9000, 256, 2), (9000, 264, 5), (5000, 520, 1), (4000, 1032, 2), (3000, 2056, 4), (2500, 4104, 2), (2000, 8200, 1),
+                                   (1000, 16392, 2), (300, 32776, 3), (20, 7168, 40)])
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_dispatch_forms(T, N, k, dt):
+    g = torch.Generator(device="cuda").manual_seed(T + N)
+    x = torch.randn((T, N), generator=g, device="cuda").to(dt)
+    rows = torch.randperm(T * k, generator=g, device="cuda").to(torch.int32).view(T, k)
+    y1, s1 = q.act_quant(x)
+    y, s = q.moe_act_quant(x, rows)
+    at = rows.view(-1).long()
+    assert torch.equal(y[at], y1.repeat_interleave(k, 0)) and torch.equal(s[at], s1.repeat_interleave(k, 0))
+
+
+@pytest.mark.parametrize("R,E", [(128, 256), (129, 256), (128, 1024), (128, 1), (4096, 300), (4097, 300), (24576, 64), (24577, 64), (65536, 848), (65537, 848), (65537, 849),
+                                 (70000, 1024), (131072, 256), (131073, 256), (300001, 40)])
+def test_blocks_forms(R, E):
+    g = torch.Generator(device="cuda").manual_seed(R + E)
+    experts = torch.randint(-1, E, (R, 1), generator=g, device="cuda", dtype=torch.int32)
+    experts[: R // 3] = torch.minimum(experts[: R // 3], torch.tensor(2, dtype=torch.int32, device="cuda"))  # some of them crowded
+    meta, rows, sizes = q.moe_block_metadata(experts, E)
+    flat = torch.where(experts.view(-1) < 0, E, experts.view(-1)).long()
+    place = torch.empty(R, dtype=torch.int64, device="cuda")
+    place[flat.sort(stable=True).indices] = torch.arange(R, device="cuda")
+    assert torch.equal(rows.view(-1).long(), torch.where(flat < E, place, -2 - place))
+    assert torch.equal(sizes.long(), torch.bincount(flat, minlength=E + 1)[:E])
+    table = q.build_block_metadata(sizes.tolist())
+    assert torch.equal(meta[: len(table)].cpu(), table) and (meta[len(table):, 2] == 0).all() and (meta[len(table):, 0] == -1).all()
+    assert len(meta) == min(R, E) + (R - min(R, E)) // 128
+
+
+@pytest.mark.parametrize("E,k,groups", [(64, 32, 1), (256, 32, 1), (1024, 32, 4), (40, 20, 2), (513, 9, 1), (512, 8, 16), (256, 3, 32)])
+@pytest.mark.parametrize("biased", [False, True])
+def test_route_where_most_logits_are_equal(E, k, groups, biased):
+    """More candidates than a warp has lanes: many equal values, and more picks than lanes that have one."""
+    g = _gen(E, k, groups)
+    logits = torch.randint(0, 2, (24, E), generator=g).float()
+    logits[0] = 0.0
+    logits[1] = 1.0
+    logits[1, E // 2] = -math.inf
+    logits[2, : E - k // 2] = -math.inf
+    logits[3] = torch.randn(E, generator=g)
+    bias = torch.zeros(E) if biased else None
+    _check_route(logits, k, bias, scoring="sigmoid", num_groups=groups, top_groups=max(1, groups // 2))
+    _check_route(logits, k, bias, scoring="softmax", num_groups=groups, top_groups=groups, renormalize=False)
+
+
+@pytest.mark.parametrize("E,k", [(60, 4), (256, 8)])
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+def test_route_of_slices(E, k, dt):
+    """Logits that start off a 16-byte boundary are read one by one: the same picks."""
+    g = torch.Generator(device="cuda").manual_seed(E)
+    logits = torch.randn((41, E), generator=g, device="cuda").to(dt)
+    shifted = torch.empty(41 * E + 1, dtype=dt, device="cuda")[1:].view(41, E)
+    shifted.copy_(logits)
+    for kw in (dict(), dict(bias=torch.randn(E, generator=g, device="cuda") * 0.1, scoring="sigmoid", num_groups=4, top_groups=2)):
+        for a, b in zip(q.moe_route(logits, k, **kw), q.moe_route(shifted, k, **kw)):
+            assert torch.equal(a, b)
+
+
+def test_route_large_bias():
+    """A bias far above the scores: c loses bits of the score, fp64 decides nearly everything."""
+    g = _gen(77)
+    logits = torch.randn(30, 64, generator=g)
+    for scoring in ("softmax", "sigmoid"):
+        _check_route(logits, 6, torch.full((64,), 1000.0), scoring=scoring)
+        _check_route(logits, 6, torch.full((64,), -3e5) + torch.randint(0, 3, (64,), generator=g), scoring=scoring, num_groups=8, top_groups=3)
