@@ -1,5 +1,6 @@
 """B200-native quantized GEMM operators (W8A8, W4A16, W4A8) behind the call signatures of the
-tile-ai/tilelang-ascend examples ``quant_batch_matmul`` and ``dequantize_gemm``.
+tile-ai/tilelang-ascend examples ``quant_batch_matmul`` and ``dequantize_gemm``, and what a mixture-of-experts layer runs
+around the grouped one (``moe``).
 
 The kernels are hand-written CUDA for sm_100a in ``csrc/`` and are reached through the C ABI of
 ``libqgemm.so`` (``include/qgemm.h``).  There is no CPU or library fallback.
