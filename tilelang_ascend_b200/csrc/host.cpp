@@ -439,8 +439,9 @@ PyObject* h_moe_route(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const int64_t k = as_int(args[1]), scoring = as_int(args[3]), groups = as_int(args[4]), top_groups = as_int(args[5]), group_top = as_int(args[6]);
   if (T == 0 || k <= 0 || k > E || scoring < 0 || groups <= 0 || top_groups <= 0 || group_top < 1 || group_top > 2) Py_RETURN_NONE;
   if (args[7] != Py_True && args[7] != Py_False) Py_RETURN_NONE;
-  if (!PyFloat_CheckExact(args[8])) Py_RETURN_NONE;
-  const float scale = (float)PyFloat_AS_DOUBLE(args[8]);
+  int64_t whole = 0;
+  if (!PyFloat_CheckExact(args[8]) && !plain_int(args[8], &whole)) Py_RETURN_NONE;
+  const float scale = PyFloat_CheckExact(args[8]) ? (float)PyFloat_AS_DOUBLE(args[8]) : (float)whole;
   const int dev = l->get_device();
   c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
   at::Tensor w = empty_cuda({T, k}, at::kFloat, dev), e = empty_cuda({T, k}, at::kInt, dev);

@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(RT_WARPS * 32, rt_min_blocks(V)) moe_route_ker
   using K = RtKey<uint32_t>;
   constexpr int L = V < 8 ? V : 8, S = V / L;  // sorted lists of a lane
   constexpr uint32_t PLACE = V - 1;            // the lowest bits of a key: V - 1 - place within the lane
-  extern __shared__ unsigned long long rt_smem[];
+  extern __shared__ __align__(16) unsigned long long rt_smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   unsigned long long* keys64 = rt_smem + (size_t)warp * p.E;
   uint32_t* keys32 = reinterpret_cast<uint32_t*>(keys64);
