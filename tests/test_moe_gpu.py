@@ -1,7 +1,8 @@
 """GPU tests of the operators around the experts' products, against plain 64-bit implementations (oracle/moe_oracle.py).
 
-Tolerances.  Picks, tables, places and int8 codes are equal.  Weights: exp and the quotients are good to 2 ulp, the sum of up to
-32 of them to 5 roundings, the factor to one: under 12 * 2^-24 < 2^-20, relative.  Combined rows: half a step of the output type, and
+Tolerances.  Picks, tables, places and int8 codes are equal.  Weights: exp and two quotients are good to 2 ulp (2 * 2^-24 each
+half), the sum of up to 32 of them to 5 roundings, the factor to one, and exp's argument l - max is off by |l - max| 2^-24 at most: under 16 * 2^-24 =
+2^-20, relative, for picks within a few units of the largest.  Combined rows: half a step of the output type, and
 for the fp32 sum of top_k products and a base (top_k + 2) * 2^-24 of the sum of the absolute values."""
 import math
 
