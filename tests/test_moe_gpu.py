@@ -694,3 +694,17 @@ def test_route_large_bias():
     for scoring in ("softmax", "sigmoid"):
         _check_route(logits, 6, torch.full((64,), 1000.0), scoring=scoring)
         _check_route(logits, 6, torch.full((64,), -3e5) + torch.randint(0, 3, (64,), generator=g), scoring=scoring, num_groups=8, top_groups=3)
+
+
+@pytest.mark.parametrize("E,groups,top_groups,k", [(160, 8, 3, 6), (348, 12, 7, 8), (1020, 17, 6, 8), (1023, 31, 30, 9), (1022, 7, 2, 16), (1000, 5, 3, 4), (90, 3, 1, 30),
+                                                   (29, 29, 11, 11), (48, 24, 20, 3), (768, 16, 4, 10)])
+@pytest.mark.parametrize("group_top", [1, 2])
+@pytest.mark.parametrize("scoring,biased,dt", [("sigmoid", True, BF16), ("softmax", False, F16), ("softmax", True, F32)])
+def test_route_groups_of_any_size(E, groups, top_groups, k, group_top, scoring, biased, dt):
+    """Groups that fill their lanes in part, and lanes of up to 60 experts."""
+    g = _gen(E, groups, group_top)
+    logits = (torch.randn(11, E, generator=g) * 1.5).to(dt)
+    logits[0, E // groups:] = -math.inf  # one group is left
+    logits[1] = 0.25
+    _check_route(logits, k, torch.randn(E, generator=g) * 0.1 if biased else None, scoring=scoring, num_groups=groups, top_groups=top_groups,
+                 group_top=group_top)

@@ -57,22 +57,29 @@ int launch_route(const qg::MoeRouteParams& p, int sms, cudaStream_t s) {
   return launch_pdl(qg::moe_route_kernel<DT, V, VEC>, (int)blocks, qg::RT_WARPS * 32, qg::rt_smem_bytes(p.E), s, p);
 }
 template <int DT, bool VEC>
-int launch_route(const qg::MoeRouteParams& p, int sms, cudaStream_t s) {
-  if (p.E <= 32) return launch_route<DT, 1, VEC>(p, sms, s);
-  if (p.E <= 64) return launch_route<DT, 2, VEC>(p, sms, s);
-  if (p.E <= 128) return launch_route<DT, 4, VEC>(p, sms, s);
-  if (p.E <= 256) return launch_route<DT, 8, VEC>(p, sms, s);
-  if (p.E <= 512) return launch_route<DT, 16, VEC>(p, sms, s);
-  return launch_route<DT, 32, VEC>(p, sms, s);
+int launch_route(const qg::MoeRouteParams& p, int v, int sms, cudaStream_t s) {
+  switch (v) {
+    case 1: return launch_route<DT, 1, VEC>(p, sms, s);
+    case 2: return launch_route<DT, 2, VEC>(p, sms, s);
+    case 4: return launch_route<DT, 4, VEC>(p, sms, s);
+    case 8: return launch_route<DT, 8, VEC>(p, sms, s);
+    case 16: return launch_route<DT, 16, VEC>(p, sms, s);
+    case 32: return launch_route<DT, 32, VEC>(p, sms, s);
+    default: return launch_route<DT, 64, false>(p, sms, s);  // some 600 experts and more in groups that leave lanes idle
+  }
 }
 template <int DT>
-int launch_route(const qg::MoeRouteParams& p, int sms, cudaStream_t s) {
-  // A lane's logits in pieces of up to 16 bytes where every row keeps that alignment and no lane has some of its experts only.
+int launch_route(qg::MoeRouteParams p, int sms, cudaStream_t s) {
+  p.log_share = 0;
+  while ((2 << p.log_share) * p.groups <= 32) ++p.log_share;
+  p.per_lane = (p.group_n + (1 << p.log_share) - 1) >> p.log_share;
   int v = 1;
-  while (32 * v < p.E) v *= 2;
+  while (v < p.per_lane) v *= 2;
+  // A lane's logits in pieces of up to 16 bytes where every row keeps that alignment and no lane has some of its places filled only.
   const int bytes = std::min(16, v * (DT == qg::RT_F32 ? 4 : 2));
-  const bool vec = p.E % v == 0 && (int64_t)p.E * (DT == qg::RT_F32 ? 4 : 2) % bytes == 0 && aligned(p.logits, bytes);
-  return vec ? launch_route<DT, true>(p, sms, s) : launch_route<DT, false>(p, sms, s);
+  const bool vec = v <= 32 && p.group_n % v == 0 && (int64_t)p.E * (DT == qg::RT_F32 ? 4 : 2) % bytes == 0 && aligned(p.logits, bytes);
+  if (vec) p.per_lane = v;
+  return vec ? launch_route<DT, true>(p, v, sms, s) : launch_route<DT, false>(p, v, sms, s);
 }
 
 // One cluster of `ctas` CTAs.

@@ -10,7 +10,8 @@
 // values are compared and a token whose decision is nearer than the error of the fp32 scores is decided again in fp64 (random
 // scores: one token in some hundreds).
 //
-// One warp per token.  A lane has V consecutive experts as 32-bit keys in the order of the values, whose lowest bits are the place within
+// One warp per token.  The experts of a group are dealt to a power of two of lanes, so that shuffles settle it whatever its size (through
+// shared memory 8000 x 160 in 8 groups was 17.3 us instead of 10.9).  A lane has up to V consecutive experts as 32-bit keys in the order of the values, whose lowest bits are the place within
 // the lane, and sorts them (in lists of eight) in registers.  The value that top_k lanes' heads reach bounds the picks from below: a
 // maximum over the heads, one redux instruction, top_k times.  The keys from there on, a dozen or so, are gathered by votes
 // and each lane counts how many come before its own.  (A maximum over the heads per pick, with a step of the winner's list, was 32
@@ -36,6 +37,7 @@ struct MoeRouteParams {
   int* experts;        // [T, k]
   long long T;
   int E, k, groups, group_n, top_groups, group_top;
+  int log_share, per_lane;  // a group's experts are dealt to 2^log_share lanes, per_lane to each
   int softmax, renormalize;
   float scale;
 };
@@ -110,47 +112,32 @@ __device__ __forceinline__ F rt_group_value(const MoeRouteParams& p, K a, K b, b
   return b > RtKey<K>::NONE ? v + w : v;
 }
 
-// The groups that stay, as a bit mask.  `keys`: this warp's c in shared memory.  P lanes share a group and keep its two largest
-// keys.  `eps` >= 0: `near` is set where the last
-// group that stays and the first that does not are no further apart than two sums of two c that may each be off by half of that.
-template <typename K>
-__device__ __forceinline__ uint32_t rt_groups(const MoeRouteParams& p, const K* keys, int lane, bool by_logits, float top,
-                                              typename RtKey<K>::F eps, bool& near) {
-  using F = typename RtKey<K>::F;
-  int share = 1;
-  while (share * 2 * p.groups <= 32) share *= 2;
-  const int g = lane / share, part = lane - g * share;
-  K a = 0, b = 0;  // largest, second largest
+// The groups that stay, as a bit mask, from the keys of all experts in shared memory.
+__device__ __forceinline__ uint32_t rt_groups_in_64(const MoeRouteParams& p, const unsigned long long* keys, int lane, bool by_logits, float top) {
+  using K = RtKey<unsigned long long>;
+  const int share = 1 << p.log_share, g = lane >> p.log_share, part = lane & (share - 1);
+  unsigned long long a = 0, b = 0;  // largest, second largest of this lane's part of group g
   if (g < p.groups) {
     for (int i = part; i < p.group_n; i += share) {
-      const K v = keys[g * p.group_n + i];
+      const unsigned long long v = keys[g * p.group_n + i];
       if (v > a) { b = a; a = v; }
       else if (v > b) b = v;
     }
   }
   for (int o = 1; o < share; o *= 2) {
-    const K a2 = __shfl_xor_sync(0xffffffffu, a, o), b2 = __shfl_xor_sync(0xffffffffu, b, o);
-    const K lo = a < a2 ? a : a2, hi2 = b > b2 ? b : b2;
-    a = a > a2 ? a : a2;
-    b = lo > hi2 ? lo : hi2;
+    const unsigned long long a2 = __shfl_xor_sync(0xffffffffu, a, o), b2 = __shfl_xor_sync(0xffffffffu, b, o);
+    b = max(max(b, b2), min(a, a2));
+    a = max(a, a2);
   }
-  const F v = rt_group_value<F>(p, a, b, by_logits, top);
-  const K mine = g < p.groups ? RtKey<K>::of(v) : 0;
+  const unsigned long long mine = g < p.groups ? K::of(rt_group_value<double>(p, a, b, by_logits, top)) : 0;
   int rank = 0;
   for (int j = 0; j < p.groups; ++j) {
-    const K other = __shfl_sync(0xffffffffu, mine, j * share);
+    const unsigned long long other = __shfl_sync(0xffffffffu, mine, j << p.log_share);
     rank += (other > mine || (other == mine && j < g)) ? 1 : 0;
   }
-  const bool leads = part == 0 && g < p.groups;
-  if (eps >= 0 && !(by_logits && p.group_top == 1)) {
-    const uint32_t last = __ballot_sync(0xffffffffu, leads && rank == p.top_groups - 1);
-    const uint32_t next = __ballot_sync(0xffffffffu, leads && rank == p.top_groups);
-    const F x = __shfl_sync(0xffffffffu, v, __ffs(last) - 1), y = __shfl_sync(0xffffffffu, v, __ffs(next) - 1);
-    if (x - y <= 2 * eps) near = true;
-  }
+  const uint32_t kept = __ballot_sync(0xffffffffu, part == 0 && g < p.groups && rank < p.top_groups);
   uint32_t stays = 0;
-  const uint32_t kept = __ballot_sync(0xffffffffu, leads && rank < p.top_groups);
-  for (int j = 0; j < p.groups; ++j) stays |= ((kept >> (j * share)) & 1u) << j;
+  for (int j = 0; j < p.groups; ++j) stays |= ((kept >> (j << p.log_share)) & 1u) << j;
   return stays;
 }
 
@@ -193,9 +180,8 @@ __device__ __noinline__ int rt_decide_in_64(const MoeRouteParams& p, const void*
   __syncwarp();
   for (int e = lane; e < p.E; e += 32) keys[e] = score.key(e);
   __syncwarp();
-  bool near = false;
   if (p.groups > 1) {
-    const uint32_t stays = rt_groups<unsigned long long>(p, keys, lane, by_logits, score.top, -1.0, near);
+    const uint32_t stays = rt_groups_in_64(p, keys, lane, by_logits, score.top);
     __syncwarp();
     for (int e = lane; e < p.E; e += 32)
       if (!((stays >> (e / p.group_n)) & 1u)) keys[e] = 0;
@@ -279,13 +265,13 @@ struct RtRow {
 #pragma unroll
     for (int i = 0; i < WORDS; ++i) w[i] = !VEC || DT == RT_F32 ? 0xff800000u : (DT == RT_BF16 ? 0xff80ff80u : 0xfc00fc00u);
   }
-  __device__ __forceinline__ void load(const void* row, int first, int E) {
+  __device__ __forceinline__ void load(const void* row, int first, int count) {
     const char* p = static_cast<const char*>(row) + (long long)first * (DT == RT_F32 ? 4 : 2);
     if constexpr (!VEC) {
 #pragma unroll
-      for (int i = 0; i < V; ++i) w[i] = first + i < E ? __float_as_uint(rt_load<DT>(row, first + i)) : 0xff800000u;
+      for (int i = 0; i < V; ++i) w[i] = i < count ? __float_as_uint(rt_load<DT>(row, first + i)) : 0xff800000u;
     } else {
-      if (first >= E) return;
+      if (count == 0) return;
       if constexpr (BYTES % 16 == 0) {
 #pragma unroll
         for (int i = 0; i < BYTES / 16; ++i) {
@@ -329,20 +315,22 @@ __global__ void __launch_bounds__(RT_WARPS * 32, rt_min_blocks(V)) moe_route_ker
   extern __shared__ __align__(16) unsigned long long rt_smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   unsigned long long* keys64 = rt_smem + (size_t)warp * p.E;
-  uint32_t* keys32 = reinterpret_cast<uint32_t*>(keys64);
   // candidates, and what is in each place of the order: (expert backwards, value)
   uint2* list = reinterpret_cast<uint2*>(rt_smem + (size_t)RT_WARPS * p.E + (RT_WARPS * p.E & 1)) + warp * RT_LIST;
   uint2* place = list + RT_LIST / 2;
-  const int first = lane * V;
+  // Lanes of a power of two to a group, so that it is settled by shuffles; in the order of the experts.
+  const int share = 1 << p.log_share, part = lane & (share - 1), my_group = lane >> p.log_share;
+  const int first = my_group * p.group_n + part * p.per_lane;
+  const int count = my_group < p.groups ? max(0, min(p.per_lane, p.group_n - part * p.per_lane)) : 0;
   const bool by_logits = p.bias == nullptr;  // the picks' order
   const bool need_sum = p.softmax && (!by_logits || !p.renormalize);
   const bool need_top = p.softmax && (need_sum || (p.groups > 1 && p.group_top == 2));
-  // Groups whose experts are those of 1, 2, 4, .. whole lanes are settled by shuffles, others through shared memory.
-  const int group_lanes = p.group_n % V == 0 ? p.group_n / V : 0;
-  const bool in_lanes = group_lanes > 0 && (group_lanes & (group_lanes - 1)) == 0;
-  const int my_group = in_lanes ? first / p.group_n : 0;
   const uint32_t below = (1u << lane) - 1u;
-  const uint32_t last_expert = 32 * V - 1, backwards = (uint32_t)(31 - lane) * V;
+  const uint32_t backwards = (uint32_t)(31 - lane) * V;
+  auto expert_of = [&](uint32_t lane_and_place) {  // both backwards
+    const int l = 31 - (int)(lane_and_place / V);
+    return (l >> p.log_share) * p.group_n + (l & (share - 1)) * p.per_lane + (int)(PLACE - (lane_and_place & PLACE));
+  };
   pdl_wait();
   pdl_launch_dependents();
   float bias[V];
@@ -350,7 +338,7 @@ __global__ void __launch_bounds__(RT_WARPS * 32, rt_min_blocks(V)) moe_route_ker
   if (!by_logits) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      bias[i] = first + i < p.E ? ld_written(p.bias + first + i) : -INFINITY;
+      bias[i] = i < count ? ld_written(p.bias + first + i) : -INFINITY;
       if (fabsf(bias[i]) < INFINITY) most_bias = fmaxf(most_bias, fabsf(bias[i]));
     }
     most_bias = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most_bias)));
@@ -360,11 +348,11 @@ __global__ void __launch_bounds__(RT_WARPS * 32, rt_min_blocks(V)) moe_route_ker
   int t = blockIdx.x * RT_WARPS + warp;
   const char* row = static_cast<const char*>(p.logits) + t * row_bytes;
   RtRow<DT, V, VEC> next;
-  if (t < p.T) next.load(row, first, p.E);
+  if (t < p.T) next.load(row, first, count);
   for (; t < p.T; t += step, row += step * row_bytes) {
     float l[V];
     next.values(l);
-    if (t + step < p.T) next.load(row + step * row_bytes, first, p.E);
+    if (t + step < p.T) next.load(row + step * row_bytes, first, count);
     float top = 0.0f, inv_sum = 1.0f;
     float c[V];
     if (need_top) {
@@ -412,27 +400,13 @@ __global__ void __launch_bounds__(RT_WARPS * 32, rt_min_blocks(V)) moe_route_ker
 #pragma unroll
     for (int i = 0; i < V; ++i) key[i / L][i % L] = (K::of(c[i]) & ~PLACE) | (PLACE - i);
     // How near two c may come before fp32 cannot tell them apart: each is off by 2^-21 of the largest score that there can be, by its
-    // rounding and by the bits of the place.  (A group's value, without a bias, is not divided by the sum.)
+    // rounding and by the bits of the place.
     const float score = p.softmax && !by_logits ? inv_sum : 1.0f;
     const float tol = 0x1p-20f * score + (0x1p-22f + V * 0x1p-22f) * (most_bias + score);
     bool near = false, kept = true;
-    if (p.groups > 1 && !in_lanes) {
-      __syncwarp();
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (first + i < p.E) keys32[first + i] = K::of(c[i]);
-      __syncwarp();
-      const uint32_t stays = rt_groups<uint32_t>(p, keys32, lane, by_logits, top, tol, near);
-      int g = first / p.group_n, at = first - g * p.group_n;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        if (first + i >= p.E || !((stays >> g) & 1u)) key[i / L][i % L] = 0u;
-        if (++at == p.group_n) { at = 0; ++g; }
-      }
-    }
 #pragma unroll
     for (int s = 0; s < S; ++s) rt_sort<L>(key[s]);
-    if (p.groups > 1 && in_lanes) {
+    if (p.groups > 1) {
       // The two largest of the group, by the exact logits where those are what is compared.
       uint32_t a = 0, b = 0;
       if (by_logits) {
@@ -451,26 +425,27 @@ __global__ void __launch_bounds__(RT_WARPS * 32, rt_min_blocks(V)) moe_route_ker
           a = max(a, key[s][0]);
         }
       }
-      for (int o = 1; o < group_lanes; o *= 2) {
+      for (int o = 1; o < share; o *= 2) {
         const uint32_t a2 = __shfl_xor_sync(0xffffffffu, a, o), b2 = __shfl_xor_sync(0xffffffffu, b, o);
         b = max(max(b, b2), min(a, a2));
         a = max(a, a2);
       }
       if (!by_logits) a = a < K::NONE ? a : a & ~PLACE, b = b < K::NONE ? b : b & ~PLACE;
       const float v = rt_group_value<float>(p, a, b, by_logits, top);
-      const bool inside = first < p.E;
+      const bool inside = my_group < p.groups;
       const uint32_t mine = inside ? K::of(v) : 0u;
-      int rank = 0;  // groups in front of mine: each of its lanes asks a share of the others
-      for (int j = lane & (group_lanes - 1); j - (lane & (group_lanes - 1)) < p.groups; j += group_lanes) {
-        const uint32_t other = __shfl_sync(0xffffffffu, mine, (j * group_lanes) & 31);
+      int rank = 0;  // groups in front of mine: each of its lanes asks some of the others
+      for (int j0 = 0; j0 < p.groups; j0 += share) {
+        const int j = j0 + part;
+        const uint32_t other = __shfl_sync(0xffffffffu, mine, (j << p.log_share) & 31);
         rank += j < p.groups && (other > mine || (other == mine && j < my_group)) ? 1 : 0;
       }
-      for (int o = 1; o < group_lanes; o *= 2) rank += __shfl_xor_sync(0xffffffffu, rank, o);
+      for (int o = 1; o < share; o *= 2) rank += __shfl_xor_sync(0xffffffffu, rank, o);
       if (!(by_logits && p.group_top == 1)) {
         const uint32_t last = __ballot_sync(0xffffffffu, inside && rank == p.top_groups - 1);
         const uint32_t behind = __ballot_sync(0xffffffffu, inside && rank == p.top_groups);
         const float x = __shfl_sync(0xffffffffu, v, __ffs(last) - 1), y = __shfl_sync(0xffffffffu, v, __ffs(behind) - 1);
-        near = x - y <= 2 * tol;
+        near = x - y <= 2 * (by_logits ? 0x1.4p-20f : tol);  // (the logits' scores are of whole logits)
       }
       kept = rank < p.top_groups;
     }
@@ -524,7 +499,7 @@ __global__ void __launch_bounds__(RT_WARPS * 32, rt_min_blocks(V)) moe_route_ker
         in_front += (((unsigned long long)more.w << 32) | more.z) > mine64;
       }
       if (lane < n) {
-        pick = (int)(last_expert - mine.x);
+        pick = expert_of(mine.x);
         rank = in_front;
       }
       if (check) {
@@ -537,7 +512,7 @@ __global__ void __launch_bounds__(RT_WARPS * 32, rt_min_blocks(V)) moe_route_ker
           if (after.y != 0) {
             close = by_logits ? mine.y == after.y : K::value(mine.y) - K::value(after.y) <= tol;
             if (close) {  // the same logit and the same bias: a tie, and in the right order
-              const int behind = (int)(last_expert - after.x);
+              const int behind = expert_of(after.x);
               if (rt_load<DT>(row, pick) == rt_load<DT>(row, behind) && (by_logits || ld_written(p.bias + pick) == ld_written(p.bias + behind))) close = false;
             }
           }
