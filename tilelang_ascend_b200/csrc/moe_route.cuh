@@ -10,13 +10,14 @@
 // values are compared and a token whose decision is nearer than the error of the fp32 scores is decided again in fp64 (random
 // scores: one token in some hundreds).
 //
-// One warp per token.  The experts of a group are dealt to a power of two of lanes, so that shuffles settle it whatever its size (through
-// shared memory 8000 x 160 in 8 groups was 17.3 us instead of 10.9).  A lane has up to V consecutive experts as 32-bit keys in the order of the values, whose lowest bits are the place within
-// the lane, and sorts them (in lists of eight) in registers.  The value that top_k lanes' heads reach bounds the picks from below: a
-// maximum over the heads, one redux instruction, top_k times.  The keys from there on, a dozen or so, are gathered by votes
-// and each lane counts how many come before its own.  (A maximum over the heads per pick, with a step of the winner's list, was 32
-// instructions a pick; this is 130 for all.)  What bounds it is issue: 16384 x 256 in bf16 with bias and groups is 1.5 us of memory and 750
-// instructions of a warp per token, 11 us at one a cycle; measured 21.7.
+// One warp per token.  The experts of a group are dealt to a power of two of lanes, so that shuffles settle it whatever its size
+// (through shared memory 8000 x 160 in 8 groups was 17.3 us instead of 10.9).  A lane has up to V consecutive experts as 32-bit keys
+// in the order of the values, whose lowest bits are the place within the lane, and sorts them (in lists of eight) in registers.  The
+// value that top_k lanes' heads reach bounds the picks from below: a maximum over the heads, one redux instruction, top_k times.  The
+// keys from there on, a dozen or so, are gathered by votes and each lane counts how many come before its own.  (A maximum over the
+// heads per pick, with a step of the winner's list, was 32 instructions a pick; this is 130 for all.)  What bounds it is issue:
+// 16384 x 256 in bf16 with bias and groups is 1.5 us of memory and 815 instructions of a warp per token, 12 us at one a cycle;
+// measured 21.7.
 #pragma once
 
 #include "common.cuh"
