@@ -1,0 +1,74 @@
+"""GPU tests of the mixture operators where fp32 does not settle the answer, and of calls at their limits, against plain 64-bit
+implementations (oracle/moe_oracle.py).
+
+Picks, codes and scales are equal.  Weights: relative 2^-20 as for ordinary logits (two ulp each of exp and two quotients, the
+sum's roundings, the factor; the differences of the logits here are exact in fp32), and 1e-37 where a weight leaves fp32's normal range."""
+import math
+
+import pytest
+import torch
+
+import tilelang_ascend_b200 as q
+from oracle import moe_oracle as mo
+from oracle import qgemm_oracle as oc
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def _gen(*seed):
+    return torch.Generator().manual_seed(sum((i + 1) * 7919 * int(s) for i, s in enumerate(seed)) % (1 << 31))
+
+
+def _check_route(logits, top_k, bias=None, **kw):
+    w, e = q.moe_route(logits.cuda(), top_k, None if bias is None else bias.cuda(), **kw)
+    w_ref, e_ref, _ = mo.route_ref(logits, top_k, bias, **kw)
+    assert torch.equal(e.cpu(), e_ref)
+    assert (w.cpu().double() - w_ref).abs().le(2.0 ** -20 * w_ref.abs() + 1e-37).all()
+    return w, e
+
+
+# ------------------------------------------------------------------------------------ routing: equal values at the last place
+def _border_rows(T, E, k, copies, base, better, g):
+    """Rows in which some experts are clearly above ``base``, ``copies`` of them are equal to it across the last place, and up to three
+    at random places are ``better`` by less than fp32 scores (or shortened keys) show; all others are clearly below."""
+    logits = base - 3.0 - torch.randint(0, 8, (T, E), generator=g).float()
+    for t in range(T):
+        order = torch.randperm(E, generator=g)
+        above, late = int(torch.randint(0, k, (1,), generator=g)), 1 + t % 3
+        logits[t, order[:above]] = base + 1.0
+        logits[t, order[above:above + copies]] = base
+        logits[t, order[above + copies:above + copies + late]] = better
+    return logits
+
+
+@pytest.mark.parametrize("E,k,copies", [(64, 1, 2), (64, 6, 7), (64, 4, 45), (256, 1, 2), (256, 8, 10), (256, 8, 60), (1024, 2, 3), (1024, 8, 9), (1024, 4, 100),
+                                        (40, 32, 33), (513, 3, 5)])
+@pytest.mark.parametrize("groups", [1, 2])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_equal_logits_in_front_of_one_a_step_above(E, k, copies, groups, scoring):
+    """fp32 logits without a bias: the places within a lane take the lowest bits of the keys, equal logits do not end the search."""
+    if E % groups or E // groups < k:
+        groups = 1
+    base = torch.tensor(1.0)
+    better = torch.nextafter(base, torch.tensor(2.0))
+    logits = _border_rows(18, E, k, copies, float(base), float(better), _gen(E, k, copies))
+    logits[0, 0] = logits[0, 1] = base
+    logits[0, 2] = better
+    _check_route(logits, k, scoring=scoring, num_groups=groups, top_groups=1, group_top=1)
+
+
+@pytest.mark.parametrize("E,k,copies", [(64, 1, 2), (64, 6, 7), (64, 4, 45), (256, 8, 10), (256, 8, 60), (1024, 8, 9), (40, 32, 33), (513, 3, 5)])
+@pytest.mark.parametrize("groups", [1, 2])
+@pytest.mark.parametrize("scoring,base,better,bias", [("sigmoid", 15.0, 15.0625, 0.0), ("sigmoid", 15.0, 15.0625, 1000.0), ("softmax", -20.0, -19.875, 0.0),
+                                                      ("sigmoid", -18.0, -17.875, 0.25)])
+@pytest.mark.parametrize("dt", [F32, BF16, F16])
+def test_route_equal_scores_in_front_of_a_near_one(E, k, copies, groups, scoring, base, better, bias, dt):
+    """One bias for all, saturated or tiny scores: a tie of logits at the last place, and behind it one that only fp64 finds larger."""
+    if E % groups or E // groups < k:
+        groups = 1
+    logits = _border_rows(12, E, k, copies, base, better, _gen(E, k, copies, groups))
+    logits[:, -1] = 0.0 if scoring == "softmax" else base - 4.0
+    assert torch.equal(logits.to(dt).float(), logits)
+    _check_route(logits.to(dt), k, torch.full((E,), bias), scoring=scoring, num_groups=groups, top_groups=1, group_top=1)

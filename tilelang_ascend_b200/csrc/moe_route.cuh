@@ -55,6 +55,12 @@ __device__ __forceinline__ float rt_load(const void* p, long long i) {
   }
 }
 
+// Two experts whose scores are the same number.
+template <int DT>
+__device__ __forceinline__ bool rt_equal(const MoeRouteParams& p, const void* row, int e, int f, bool by_logits) {
+  return rt_load<DT>(row, e) == rt_load<DT>(row, f) && (by_logits || ld_written(p.bias + e) == ld_written(p.bias + f));
+}
+
 // The larger value, or NaN if either is one.
 __device__ __forceinline__ float rt_max(float a, float b) {
   float v;
@@ -504,19 +510,15 @@ __global__ void __launch_bounds__(RT_WARPS * 32, rt_min_blocks(V)) moe_route_ker
         rank = in_front;
       }
       if (check) {
-        if (rank <= p.k) place[rank] = mine;
-        if (lane == 0) place[32] = make_uint2(0u, 0u);  // (32 candidates at most: nothing is in that place)
+        // Each candidate against the one in front of it, those behind the last pick against that pick: a run of equal ones across the
+        // last place may hide one that is larger.
+        if (rank < p.k) place[rank] = mine;
         __syncwarp();
         bool close = false;
-        if (rank < p.k && pick >= 0) {
-          const uint2 after = place[rank + 1];
-          if (after.y != 0) {
-            close = by_logits ? mine.y == after.y : K::value(mine.y) - K::value(after.y) <= tol;
-            if (close) {  // the same logit and the same bias: a tie, and in the right order
-              const int behind = expert_of(after.x);
-              if (rt_load<DT>(row, pick) == rt_load<DT>(row, behind) && (by_logits || ld_written(p.bias + pick) == ld_written(p.bias + behind))) close = false;
-            }
-          }
+        if (lane < n && rank > 0) {
+          const uint2 front = place[min(rank, p.k) - 1];
+          close = by_logits ? mine.y == front.y : K::value(front.y) - K::value(mine.y) <= tol;
+          if (close) close = !rt_equal<DT>(p, row, expert_of(front.x), pick, by_logits);  // a tie is in the right order
         }
         if (__any_sync(0xffffffffu, close)) rank = rt_rank_in_64(p, row, DT, by_logits, pick, n, lane);
       }
@@ -542,7 +544,24 @@ __global__ void __launch_bounds__(RT_WARPS * 32, rt_min_blocks(V)) moe_route_ker
         const int e = __shfl_sync(0xffffffffu, first + (int)(PLACE - (head & PLACE)), first_owner);
         if (check && r > 0 && (by_logits ? m == last : K::value(last) - K::value(m) <= tol)) {
           const int f = __shfl_sync(0xffffffffu, pick, r - 1);
-          near = !(rt_load<DT>(row, e) == rt_load<DT>(row, f) && (by_logits || ld_written(p.bias + e) == ld_written(p.bias + f)));
+          if (r < p.k) {
+            near = !rt_equal<DT>(p, row, e, f, by_logits);
+          } else {  // behind the last pick: all that are left
+            constexpr int HALF = V > 32 ? V / 2 : V;  // places to a mask
+#pragma unroll
+            for (int h = 0; h < V; h += HALF) {
+              uint32_t left = 0;  // those of this lane that come as near
+#pragma unroll
+              for (int s = 0; s < HALF / L; ++s)
+#pragma unroll
+                for (int i = 0; i < L; ++i) {
+                  const uint32_t of = key[h / L + s][i], v = of & ~PLACE;
+                  if (by_logits ? v == last : K::value(last) - K::value(v) <= tol) left |= 1u << (PLACE - (of & PLACE) - h);
+                }
+              for (; left != 0 && !near; left &= left - 1) near = !rt_equal<DT>(p, row, first + h + __ffs(left) - 1, f, by_logits);
+            }
+            near = __any_sync(0xffffffffu, near);
+          }
         }
         last = m;
         if (r == p.k) break;
