@@ -72,3 +72,21 @@ def test_route_equal_scores_in_front_of_a_near_one(E, k, copies, groups, scoring
     logits[:, -1] = 0.0 if scoring == "softmax" else base - 4.0
     assert torch.equal(logits.to(dt).float(), logits)
     _check_route(logits.to(dt), k, torch.full((E,), bias), scoring=scoring, num_groups=groups, top_groups=1, group_top=1)
+
+
+# ---------------------------------------------------------------------------- routing: groups whose sums leave fp32's range
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_route_groups_of_huge_biases(scoring):
+    """Two biases that fp32 holds and whose sum it does not: groups worth 6.0e38 and 6.4e38, and a group masked by fp32's lowest
+    number beside one that offers nothing."""
+    logits = torch.randn(6, 16, generator=_gen(1))
+    bias = torch.zeros(16)
+    bias[0:4], bias[8:12] = 3.0e38, 3.2e38
+    _, e = _check_route(logits, 4, bias, scoring=scoring, num_groups=4, top_groups=1)
+    assert ((e >= 8) & (e < 12)).all()
+    bias = torch.full((16,), torch.finfo(F32).min)
+    logits[:, :8] = -math.inf
+    _, e = _check_route(logits, 3, bias, scoring=scoring, num_groups=2, top_groups=1)
+    assert (e >= 8).all()
+    logits[3:] = -math.inf
+    _check_route(logits, 3, bias, scoring=scoring, num_groups=2, top_groups=1)

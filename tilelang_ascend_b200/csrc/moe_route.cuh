@@ -452,7 +452,8 @@ __global__ void __launch_bounds__(RT_WARPS * 32, rt_min_blocks(V)) moe_route_ker
         const uint32_t last = __ballot_sync(0xffffffffu, inside && rank == p.top_groups - 1);
         const uint32_t behind = __ballot_sync(0xffffffffu, inside && rank == p.top_groups);
         const float x = __shfl_sync(0xffffffffu, v, __ffs(last) - 1), y = __shfl_sync(0xffffffffu, v, __ffs(behind) - 1);
-        near = x - y <= 2 * (by_logits ? 0x1.4p-20f : tol);  // (the logits' scores are of whole logits)
+        const float off = 2 * (by_logits ? 0x1.4p-20f : tol);  // (the logits' scores are of whole logits)
+        near = most_bias < 0x1p126f ? x - y <= off : !(x - y > off);  // two sums may both be beyond fp32
       }
       kept = rank < p.top_groups;
     }
