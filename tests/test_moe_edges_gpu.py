@@ -90,3 +90,16 @@ def test_route_groups_of_huge_biases(scoring):
     assert (e >= 8).all()
     logits[3:] = -math.inf
     _check_route(logits, 3, bias, scoring=scoring, num_groups=2, top_groups=1)
+
+
+# --------------------------------------------------------------------------------------------- routing: weights of small scores
+@pytest.mark.parametrize("picked", [(-29.0, -88.0), (-29.0, -88.0, -100.0), (0.0, -60.0), (-31.0, -90.0, -110.0), (-20.0, -29.5, -30.5, -95.0), (3.0, -31.0, -86.0),
+                                    (90.0, -40.0), (-29.0, -29.0, -105.0), (-2000.0, -2001.0), (-5.0, -700.0)])
+def test_route_sigmoid_weights_of_small_scores(picked):
+    """Divided by their sum, scores that sigmoid takes out of fp32's range still have weights in it."""
+    logits = torch.full((3, 64), -math.inf)
+    for t in range(3):
+        logits[t, torch.randperm(64, generator=_gen(t, len(picked)))[:len(picked)]] = torch.tensor(picked)
+    _check_route(logits, len(picked), scoring="sigmoid")
+    _check_route(logits, len(picked) + 2, scoring="sigmoid", scale=2.5)
+    _check_route(logits, len(picked), scoring="sigmoid", renormalize=False)
