@@ -370,8 +370,9 @@ int qgemm_moe_route(const void* logits, const float* bias, float* weights, int32
  *   block_metadata = (expert, first row, valid rows) of every block of up to block_M rows     int32 [blocks, 3]
  * as construct_inputs builds the table (example_grouped_gemm_fwd.py:147-166).  blocks = qgemm_moe_block_count(): what
  * the picks can need at most; entries without a block are (-1, entries, 0), which qgemm_w8a8_grouped skips.
- * num_experts <= 1024, block_M <= 128.
+ * num_experts <= 1024, block_M <= 128, entries <= 2^30, blocks <= QGEMM_MOE_MAX_BLOCKS (qgemm_w8a8_grouped takes 2^24).
  */
+#define QGEMM_MOE_MAX_BLOCKS 715827882 /* the table's values are addressed by 32-bit indexes */
 int64_t qgemm_moe_block_count(int64_t entries, int64_t num_experts, int64_t block_M);
 int qgemm_moe_blocks(const int32_t* experts, int32_t* block_metadata, int32_t* rows, int32_t* sizes, int64_t entries,
                      int64_t num_experts, int64_t block_M, void* stream);

@@ -156,6 +156,8 @@ int qgemm_moe_blocks(const int32_t* experts, int32_t* block_metadata, int32_t* r
   if (entries < 0 || entries > (1ll << 30)) return fail("qgemm_moe_blocks: 0 to 2^30 entries (got %lld)", (long long)entries);
   if (num_experts < 1 || num_experts > qg::MB_MAX_E) return fail("qgemm_moe_blocks: 1 to %d experts (got %lld)", qg::MB_MAX_E, (long long)num_experts);
   if (block_M < 1 || block_M > 128) return fail("qgemm_moe_blocks: block_M must be 1 to 128 (got %lld)", (long long)block_M);
+  if (qgemm_moe_block_count(entries, num_experts, block_M) > QGEMM_MOE_MAX_BLOCKS)
+    return fail("qgemm_moe_blocks: no more than %d blocks (got %lld entries in blocks of %lld)", QGEMM_MOE_MAX_BLOCKS, (long long)entries, (long long)block_M);
   if (sizes == nullptr || (entries > 0 && (experts == nullptr || block_metadata == nullptr || rows == nullptr)))
     return fail("qgemm_moe_blocks: null pointer");
   if (!aligned(experts, 4) || !aligned(block_metadata, 4) || !aligned(rows, 4) || !aligned(sizes, 4))
