@@ -391,7 +391,8 @@ int qgemm_moe_act_quant(const void* X, const int32_t* rows, int8_t* Y, float* S,
  *   a[m, f] = silu(X[m, f]) * X[m, F + f]        silu(g) = g / (1 + exp(-g))
  *   S[m]    = max(max_f |a[m, f]|, 1e-4) / 127   rounded to fp32 (round_scale != 0: then up to a power of two)
  *   Y[m, f] = int8( a[m, f] / S[m] to the nearest integer )
- * with a and the quotient exact: where fp32 cannot tell which integer is nearer, fp64 decides.  In a row with an infinity or a NaN
+ * with a and the quotient exact, over the whole range of X's type: where fp32 cannot tell which integer is nearer, or does not hold
+ * the products, fp64 decides.  Where max|a| / 127 is beyond fp32 S is an infinity and Y unspecified; in a row with an infinity or a NaN
  * S is one and Y unspecified.  X 16-byte, Y 8-byte aligned, F % 8 == 0.
  */
 int qgemm_swiglu_act_quant(const void* X, int8_t* Y, float* S, int64_t M, int64_t F, int x_dtype, int round_scale,

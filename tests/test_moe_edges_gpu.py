@@ -103,3 +103,50 @@ def test_route_sigmoid_weights_of_small_scores(picked):
     _check_route(logits, len(picked), scoring="sigmoid")
     _check_route(logits, len(picked) + 2, scoring="sigmoid", scale=2.5)
     _check_route(logits, len(picked), scoring="sigmoid", renormalize=False)
+
+
+# --------------------------------------------------------------------------------------- gate and quantise: bf16's whole range
+def _far_rows(M, F, g):
+    """Every third row has products that fp32 does not hold: gates below -87 beside ups of 1e29 and more, or products above 3.4e38."""
+    x = torch.randn(M, 2 * F, generator=g) * 2
+    for m in range(0, M, 3):
+        kind, at = (m // 3) % 6, int(torch.randint(0, F, (1,), generator=g))
+        if kind == 0:
+            x[m, at], x[m, F + at] = -90.0, 1e38
+        elif kind == 1:
+            x[m] *= 1e18
+            x[m, at] = x[m, F + at] = 1e20
+        elif kind == 2:
+            x[m, :F] = -87.0 - 15 * torch.rand(F, generator=g)
+            x[m, F:] = torch.where(torch.rand(F, generator=g) < 0.5, 1e38, -1e38) * torch.rand(F, generator=g)
+        elif kind == 3:
+            x[m, at], x[m, F + at] = -87.5, 2.5e29
+        elif kind == 4:
+            x[m, :F], x[m, F:] = 1.5e19, torch.where(torch.rand(F, generator=g) < 0.5, 2e20, -2e20)
+        else:
+            x[m, at], x[m, F + at] = 3e30, -3e30  # 9e60 / 127: beyond fp32, the scale is an infinity
+    return x.to(BF16)
+
+
+@pytest.mark.parametrize("M,F", [(18, 8), (19, 264), (40, 2048), (20, 2056), (21, 4104), (18, 8200), (18, 16392), (18, 33000), (1500, 256), (3000, 2056), (1300, 7168)])
+@pytest.mark.parametrize("round_scale", [False, True])
+def test_gate_over_the_whole_range_of_bf16(M, F, round_scale):
+    x = _far_rows(M, F, _gen(M, F))
+    assert torch.isfinite(x.float()).all()
+    y, s = [t.cpu() for t in q.swiglu_act_quant(x.cuda(), round_scale)]
+    y_ref, s_ref = [t.cpu() for t in mo.swiglu_act_quant_ref(x.cuda(), round_scale)]
+    there = torch.isfinite(mo.swiglu_act_quant_ref(x.cuda())[1].cpu()).view(-1)
+    assert torch.equal(s[there], s_ref[there]) and torch.equal(y[there], y_ref[there])
+    assert (s[~there] == math.inf).all() and int((~there).sum()) == len(range(15, M, 18))
+
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("F", [264, 4104, 33000])
+def test_gate_infinities_beside_far_products(value, F):
+    """An infinity or a NaN among the inputs keeps the row's scale from being a number, whatever the others are."""
+    x = _far_rows(24, F, _gen(F))
+    want = [t.cpu() for t in q.swiglu_act_quant(x.cuda())]
+    x[6, 3] = x[9, F + 7] = x[12, F - 1] = value
+    y, s = [t.cpu() for t in q.swiglu_act_quant(x.cuda())]
+    assert not torch.isfinite(s[[6, 9, 12]]).any()
+    keep = [m for m in range(24) if m not in (6, 9, 12, 15)]
+    assert torch.equal(y[keep], want[0][keep]) and torch.equal(s[keep], want[1][keep])

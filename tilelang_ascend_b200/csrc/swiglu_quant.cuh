@@ -9,11 +9,17 @@
 //
 // What fp32 makes of a, relative: 2^-22 by ex2.approx, |g| 7.5e-8 by the rounding of its argument where g < 0 (where g > 0 the factor
 // e / (1 + e) takes it down to 2e-8), 2^-24 by the sum, 2^-23 by rcp.approx, 2^-23 by two products: 5.4e-7 + 7.5e-8 max(0, -g).  The
-// quotient by s adds 2.4e-7.  (For g < -87 fp32 gives 0 where a is up to 1e-36 |u|: right as long as |u| < 1e29.)
+// quotient by s adds 2.4e-7.
+//
+// bf16 has products that fp32 has not: below g = -87 its sigmoid is 0, which |u| of 2^96 and more brings back into the range of codes, and
+// |g u| goes up to 1e77, whose 127th part may still be an fp32 number.  Both show in what a row's reductions give anyway (the lowest gate, a
+// maximum that is no number); such a row is looked through again and, where it has to be, done in fp64 as a whole.
 //
 // 4 F bytes in and F out per row.  A row is held in registers as fp32 between its maximum and its codes.  Pairs of values go through
 // the packed fp32 instructions; two MUFU operations per element are the next bound behind memory.
 #pragma once
+
+#include <type_traits>
 
 #include "act_quant.cuh"
 #include "common.cuh"
@@ -121,6 +127,43 @@ __device__ __noinline__ uint2 sq_codes64(const uint4* gp, const uint4* up, float
   return codes;
 }
 
+// A row whose lowest gate or largest product says that fp32 may not hold its products: where its inputs are numbers, and one of them is
+// large enough for that, every element again in fp64.  An infinite scale (max|a| / 127 beyond fp32) gives codes of 0.
+template <int TPR>
+__device__ __noinline__ void sq_far_row(const uint4* x, int chunks, int t, int round_scale, uint32_t* largest, uint2* y, float* s) {
+  uint32_t m2 = 0;  // largest magnitude, as bits of bf16
+  for (int c = t; c < chunks; c += TPR) {
+    const uint4 g = ld_written(x + c), u = ld_written(x + chunks + c);
+    const uint32_t M = 0x7fff7fffu;
+    m2 = __vimax3_u16x2(__vimax3_u16x2(m2, g.x & M, g.y & M), g.z & M, g.w & M);
+    m2 = __vimax3_u16x2(__vimax3_u16x2(m2, u.x & M, u.y & M), u.z & M, u.w & M);
+  }
+  const uint32_t most = max(m2 & 0xffffu, m2 >> 16);
+  int no_number = most >= 0x7f80u, far = most >= 0x5f80u;  // 0x5f80: 2^64
+  if constexpr (TPR > 32) {
+    no_number = __syncthreads_or(no_number);
+    far = __syncthreads_or(far);
+  } else {
+    no_number = __any_sync(0xffffffffu, no_number);
+    far = __any_sync(0xffffffffu, far);
+  }
+  if (no_number || !far) return;
+  double best = 1e-4;
+  for (int c = t; c < chunks; c += TPR) best = fmax(best, sq_largest64<true>(x + c, x + chunks + c, 0xffu));
+  uint32_t bits = __float_as_uint((float)(best * (1.0 / 127.0)));
+  if constexpr (TPR > 32) {
+    atomicMax(largest, bits);
+    __syncthreads();
+    bits = *largest;
+  } else {
+    bits = __reduce_max_sync(0xffffffffu, bits);
+  }
+  float scale = __uint_as_float(bits);
+  if (round_scale) scale = aq_pow2_ceil(scale);
+  if (t == 0) *s = scale;
+  for (int c = t; c < chunks; c += TPR) y[c] = sq_codes64<true>(x + c, x + chunks + c, scale, 0xffu, make_uint2(0u, 0u));
+}
+
 // TPR threads share a row, KEEP chunks of eight elements of it in each one's registers; longer rows are computed again for their codes.
 // The blocks are persistent: the next row's loads are issued when this one's values are in fp32, and are in flight while its
 // maximum is settled and its codes are stored.
@@ -140,13 +183,17 @@ __global__ void __launch_bounds__(sq_block(TPR), sq_min_blocks(TPR, KEEP)) swigl
   constexpr int ROWS = sq_block(TPR) / TPR;
   constexpr int WPR = TPR / 32;  // warps per row
   static_assert(WPR == 1 || ROWS == 1, "barriers are of the whole block");
+  // Eight chunks in 128 registers: a row's number is 32 bits wide (2^31 rows of 3592 elements and more are beyond any memory), the
+  // addresses are not kept.  8000 x 4096 34.0 us, otherwise 35.8.
+  constexpr bool TIGHT = KEEP == 8 && TPR > 32;
+  using Row = std::conditional_t<TIGHT, int, long long>;
   __shared__ uint32_t red[2][WPR];
   __shared__ uint32_t largest[2];  // scales as bits, of this row and the next one
   const int t = threadIdx.x % TPR;
   const int warp = threadIdx.x >> 5;
   const int chunks = p.F >> 3;
-  const long long step = (long long)gridDim.x * ROWS;
-  long long row = (long long)blockIdx.x * ROWS + threadIdx.x / TPR;
+  const Row step = (Row)gridDim.x * ROWS;
+  Row row = (Row)blockIdx.x * ROWS + threadIdx.x / TPR;
   if (WPR > 1 && t == 0) largest[0] = 0u;
   // a thread copies its own chunks into its own slots, so that no barrier is needed to read them
   extern __shared__ uint4 sq_slots[];
@@ -155,8 +202,8 @@ __global__ void __launch_bounds__(sq_block(TPR), sq_min_blocks(TPR, KEEP)) swigl
 #pragma unroll
   for (int i = 0; i < KEEP; ++i)
     if (t + i * TPR >= chunks) slot[2 * i * BLOCK] = slot[(2 * i + 1) * BLOCK] = make_uint4(0u, 0u, 0u, 0u);
-  auto load = [&](long long of) {
-    const uint4* x = p.X + of * 2 * chunks;
+  auto load = [&](Row of) {
+    const uint4* x = p.X + (long long)of * 2 * chunks;
     if (of < p.M) {
 #pragma unroll
       for (int i = 0; i < KEEP; ++i) {
@@ -169,9 +216,9 @@ __global__ void __launch_bounds__(sq_block(TPR), sq_min_blocks(TPR, KEEP)) swigl
     }
   };
   load(row);
-  const f32x2 magic = f2_make(12582912.0f, 12582912.0f), unmagic = f2_make(-12582912.0f, -12582912.0f);
+  const f32x2 magic = f2_make(12582912.0f, 12582912.0f);
   for (int turn = 0; row < p.M; row += step, turn ^= 1) {
-    const uint4* x = p.X + row * 2 * chunks;
+    const uint4* x = p.X + (long long)row * 2 * chunks;
     f32x2 a[KEEP][4];
     float most[KEEP], top = 0.0f;  // |a|: of a chunk, of this thread
     uint32_t low2 = 0;             // the lowest gates of this thread, as bits: negative numbers are the larger the lower they are
@@ -208,13 +255,14 @@ __global__ void __launch_bounds__(sq_block(TPR), sq_min_blocks(TPR, KEEP)) swigl
       if (t == 0) largest[turn ^ 1] = 0u;  // everybody is through with the last row's
     }
     const bool finite = m < 0x7f800000u;
+    const bool odd = BF16 && (!finite || low > 0xc2aeu);  // 0xc2ae: -87
     float lowest = 0.0f;  // max(0, -g) over the row; beyond 88 fp32 gives 0 for a
     if (low & 0x8000u) lowest = fminf(BF16 ? __uint_as_float((low & 0x7fffu) << 16) : __half2float(__ushort_as_half((unsigned short)(low & 0x7fffu))), 88.0f);
     const float off = 5.5e-7f + 7.5e-8f * lowest;
     const float from = __uint_as_float(m) * (1.0f - (2.0f * off + 2e-7f));
     double best = 0.0;
     // Whoever may be the largest: nearly always one element of one thread, whose gate and up are kept over the next row's loads.
-    uint32_t only = 0, only_g = 0, only_u = 0;
+    uint32_t only = 0;  // (gate, up): not both zero
     const bool may = finite && m != 0 && top >= from;
     if (may) {
       auto consider = [&](const uint4* gp, const uint4* up, const f32x2 (&v)[4]) {
@@ -226,10 +274,8 @@ __global__ void __launch_bounds__(sq_block(TPR), sq_min_blocks(TPR, KEEP)) swigl
           marked |= (fabsf(lo) >= from ? 1u << (2 * i) : 0u) | (fabsf(hi) >= from ? 2u << (2 * i) : 0u);
         }
         if (only == 0 && (marked & (marked - 1)) == 0) {
-          only = marked;
           const int i = __ffs(marked) - 1;
-          only_g = reinterpret_cast<const volatile uint16_t*>(gp)[i];
-          only_u = reinterpret_cast<const volatile uint16_t*>(up)[i];
+          only = reinterpret_cast<const volatile uint16_t*>(gp)[i] | (uint32_t)reinterpret_cast<const volatile uint16_t*>(up)[i] << 16;
         } else {
           best = fmax(best, sq_largest64<BF16>(gp, up, marked));
         }
@@ -244,7 +290,7 @@ __global__ void __launch_bounds__(sq_block(TPR), sq_min_blocks(TPR, KEEP)) swigl
       }
     }
     load(row + step);  // every slot has been read
-    if (only != 0) best = fmax(best, fabs(sq_gate64(sq_float<BF16>(only_g), sq_float<BF16>(only_u))));
+    if (only != 0) best = fmax(best, fabs(sq_gate64(sq_float<BF16>(only & 0xffffu), sq_float<BF16>(only >> 16))));
     // The scale of each candidate, as bits; rounding keeps the order, so that the largest is the row's.
     uint32_t bits = __float_as_uint((float)(fmax(best, 1e-4) * (1.0 / 127.0)));
     if (WPR > 1) {
@@ -260,15 +306,15 @@ __global__ void __launch_bounds__(sq_block(TPR), sq_min_blocks(TPR, KEEP)) swigl
     if (t == 0) p.S[row] = scale;
     const float rcp = sq_rcp(scale);
     const float share = finite ? rcp * (off + 2.5e-7f) : 0.0f;  // what a quotient may be off by, per |a|
-    uint2* y = reinterpret_cast<uint2*>(p.Y) + row * chunks;
-    const f32x2 rcp2 = f2_make(rcp, rcp), less_rcp2 = f2_make(-rcp, -rcp);
+    uint2* y = reinterpret_cast<uint2*>(p.Y) + (long long)row * chunks;
+    const f32x2 rcp2 = f2_make(rcp, rcp);
     auto store = [&](int c, const f32x2 (&v)[4], float m) {
       float f[8], d[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const f32x2 s = f2_fma(v[i], rcp2, magic);  // 1.5 * 2^23 + a / s: the low bits are the nearest integer
         f2_get(s, f[2 * i], f[2 * i + 1]);
-        f2_get(f2_fma(v[i], less_rcp2, f2_add(s, unmagic)), d[2 * i], d[2 * i + 1]);  // how far it is
+        f2_get(f2_fma(v[i], rcp2, f2_sub(magic, s)), d[2 * i], d[2 * i + 1]);  // how far it is
       }
       uint2 codes = make_uint2(aq_pack4(f), aq_pack4(f + 4));
       const float sure = 0.5f - m * share;
@@ -293,6 +339,12 @@ __global__ void __launch_bounds__(sq_block(TPR), sq_min_blocks(TPR, KEEP)) swigl
       f32x2 v[4];
       sq_gate8<BF16>(ld_written(x + c), ld_written(x + chunks + c), v);
       store(c, v, __uint_as_float(m));
+    }
+    if (odd) {
+      Row again = row;
+      if constexpr (TIGHT) asm volatile("" : "+r"(again));  // the addresses are computed once more, not kept until here
+      const long long r = again;
+      sq_far_row<TPR>(p.X + r * 2 * chunks, chunks, t, p.round_scale, &largest[turn], reinterpret_cast<uint2*>(p.Y) + r * chunks, p.S + r);
     }
   }
 }

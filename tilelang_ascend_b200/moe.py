@@ -132,7 +132,8 @@ def swiglu_act_quant(x, round_scale: bool = False, stream=None):
 
     ``a = silu(gate) * up``; ``scale = max(max |a|, 1e-4) / 127`` in fp32 (a power of two not below it when ``round_scale``);
     ``y`` the integer nearest to ``a / scale``.  Both are those of the exact ``a``: no rounding of the product to 16 bits lies
-    between, and values next to a border are decided in 64 bits."""
+    between, and values next to a border, or beyond what 32 bits hold, are decided in 64 bits.  A row with an infinity or a NaN, or whose
+    scale is beyond float32, has no number for its scale and unspecified ``y``."""
     if stream is None:
         ys = (ops._host or ops._native()).swiglu_act_quant(x, round_scale)
         if ys is not None:
