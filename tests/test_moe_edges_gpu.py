@@ -150,3 +150,55 @@ def test_gate_infinities_beside_far_products(value, F):
     assert not torch.isfinite(s[[6, 9, 12]]).any()
     keep = [m for m in range(24) if m not in (6, 9, 12, 15)]
     assert torch.equal(y[keep], want[0][keep]) and torch.equal(s[keep], want[1][keep])
+
+
+# ------------------------------------------------------------------- the grouped product over tables as long as the worst one
+@pytest.mark.parametrize("sizes,K,N", [((300,), 272, 528), ((700, 513), 144, 2064), ((1000, 385, 257), 272, 4096), ((1,) * 16, 528, 4112), ((129,) * 11 + (81,), 400, 2048),
+                                       ((0, 5, 0), 144, 272)])
+@pytest.mark.parametrize("layout", ["KN", "NK"])
+def test_grouped_product_over_host_built_tables_of_the_worst_length(sizes, K, N, layout):
+    """Tables that the host built and that are as long as one made on the device: against the oracle, and with entries added."""
+    g = torch.Generator(device="cuda").manual_seed(K + N)
+    G, R = len(sizes), sum(sizes)
+    A = torch.randint(-128, 128, (R, K), dtype=torch.int8, generator=g, device="cuda")
+    B = torch.randint(-128, 128, (G, K, N) if layout == "KN" else (G, N, K), dtype=torch.int8, generator=g, device="cuda")
+    s, sa = torch.rand((G, N), generator=g, device="cuda"), torch.rand(R, generator=g, device="cuda")
+    table = q.build_block_metadata(sizes, 128)
+    worst = min(R, G) + (R - min(R, G)) // 128
+    if 0 not in sizes:
+        assert len(table) == worst
+    kw = dict(out_dtype=BF16, b_layout=layout)
+    ref = torch.zeros(R, N, dtype=torch.int32, device="cuda")
+    at = 0
+    for i, n in enumerate(sizes):
+        b = B[i].double() if layout == "KN" else B[i].double().t()
+        ref[at:at + n] = (A[at:at + n].double() @ b).to(torch.int32)  # exact: below 2^53
+        at += n
+    got, acc = q.grouped_quant_matmul(A, B, table.cuda(), s, sa, return_accumulators=True, **kw)
+    assert torch.equal(acc, ref)
+    more = torch.cat([table, torch.tensor([[-1, R, 0]], dtype=torch.int32).repeat(worst, 1)]).cuda()
+    assert torch.equal(q.grouped_quant_matmul(A, B, more, s, sa, **kw), got)
+    assert torch.equal(q.grouped_quant_matmul(A, B, table.cuda(), s, sa, **kw), got)
+
+
+@pytest.mark.parametrize("K,N,layout", [(144, 4096, "KN"), (272, 2048, "NK"), (16, 1040, "KN")])
+def test_grouped_product_of_many_entries_per_cta(K, N, layout):
+    """More items than 32 for every CTA, most of them without rows, in runs of any length."""
+    g = _gen(K, N)
+    sizes = [int(v) for v in torch.randint(0, 200, (64,), generator=g)]
+    G, R = len(sizes), sum(sizes)
+    A = torch.randint(-128, 128, (R, K), dtype=torch.int8, generator=g).cuda()
+    B = torch.randint(-128, 128, (G, K, N) if layout == "KN" else (G, N, K), dtype=torch.int8, generator=g).cuda()
+    s, sa = torch.rand((G, N), generator=g).cuda(), torch.rand(R, generator=g).cuda()
+    used = q.build_block_metadata(sizes, 128)
+    want = q.grouped_quant_matmul(A, B, used.cuda(), s, sa, out_dtype=BF16, b_layout=layout)
+    none = torch.tensor([[-1, R, 0], [0, 0, 0], [3, R, 4]], dtype=torch.int32)
+    for longest in (20, 300):
+        pieces = []
+        for entry in used:
+            n = int(torch.randint(0, longest, (1,), generator=g))
+            pieces += [none[torch.randint(0, 3, (n,), generator=g)], entry[None]]
+        table = torch.cat(pieces + [none[:1].repeat(900, 1)])
+        assert len(table) * ((N + 255) // 256) > 32 * 148
+        got = q.grouped_quant_matmul(A, B, table.cuda(), s, sa, out_dtype=BF16, b_layout=layout)
+        assert torch.equal(got, want)

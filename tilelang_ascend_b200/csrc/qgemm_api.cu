@@ -812,8 +812,9 @@ static int w8a8_impl(const int8_t* A, const int8_t* B, const float* scale_b, con
     if (nk) return bf ? launch_w8_clusters<true, true, form>(tmA, tmB, tmC, p, grid, s) : launch_w8_clusters<true, false, form>(tmA, tmB, tmC, p, grid, s);
     return bf ? launch_w8_clusters<false, true, form>(tmA, tmB, tmC, p, grid, s) : launch_w8_clusters<false, false, form>(tmA, tmB, tmC, p, grid, s);
   }
-  // A table with as many entries as its rows can need at most: from qgemm_moe_blocks, and probably not all in use.
-  const bool skip = meta != nullptr && num_blocks >= qgemm_moe_block_count(M, batch, qg::W8_BM);
+  // A table with as many entries as its rows can need at most may be from qgemm_moe_blocks and have some without rows, which its form
+  // passes over.  Where every CTA has one item only there is little to gain, and one group alone fills such a table.
+  const bool skip = meta != nullptr && batch > 1 && p.num_items > grid && num_blocks >= qgemm_moe_block_count(M, batch, qg::W8_BM);
   if (BN == 256) {
     if (nk) return bf ? launch_w8<256, true, true>(tmA, tmB, tmC, p, grid, s, skip) : launch_w8<256, true, false>(tmA, tmB, tmC, p, grid, s, skip);
     return bf ? launch_w8<256, false, true>(tmA, tmB, tmC, p, grid, s, skip) : launch_w8<256, false, false>(tmA, tmB, tmC, p, grid, s, skip);

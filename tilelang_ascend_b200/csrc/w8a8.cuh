@@ -179,9 +179,11 @@ __device__ __forceinline__ void w8_zero_uncovered(const W8A8Params& p, int warp4
 // 79, 1.9 GB from L2 into the SMs instead of 2.8), 16 x 512 x 7168 x 2048 [N, K] 101 -> 89.  Which shapes take it: w8_pair_pays in qgemm_api.cu.
 //
 // SKIP: for tables with entries that have no rows (one that was made on the device has as many entries as its picks could need): all three
-// roles pass over their items.  us, without / with it: 16 tokens to 4 of 64 experts, 7168 x 4096, 44 of 64 entries in use 229 / 198; 4096
-// tokens, 4096 x 2048, 158 of 191 184 / 150.  A form of its own, because the look-up in the MMA warp costs 1 - 3 % of a call
-// whose table has none, 14 % of 1500 rows in 12 groups, 4096 x 1024.
+// roles pass over their items.  The MMA warp looks up which of the CTA's next 32 items have rows, one per lane, before the first of them
+// (at the start beside the first loads); a look-up per item in its k loop cost calls whose table has no such entry up to 6 %.  us,
+// without / with it: 16 tokens to 4 of 64 experts, 7168 x 4096, 45 of 64 entries in use 230 / 205; 4096 tokens to 2 of 64, 4096 x 2048,
+// 95 of 127 133 / 117; every entry in use: 1213 rows in two groups, 4096 x 2048 19.9 / 19.9, 1500 in 12, 1024 x 4096 16.5 / 16.6, a
+// token to 4 of 64, 7168 x 2048, one item per CTA 27.2 / 27.6, not taken.
 template <int BN, bool B_NK, bool OUT_BF16, W8Form FORM = W8_ALONE, bool SKIP = false>
 __global__ void __launch_bounds__(W8_THREADS, 1)
 w8a8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
@@ -337,17 +339,19 @@ w8a8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     uint32_t phase = 0;
     int it = 0;
     bool ok = true;
-    auto empty_item = [&](int item) {  // (the vote tells the compiler that the warp stays together)
-      return SKIP && item < p.num_items && __any_sync(0xffffffffu, w8_tile<PAIR>(p, item, crank).rows <= 0);
-    };
-    bool nothing_next = empty_item(tile_first);  // there is nothing to do for the next item
+    uint32_t to_do = 0;  // of this and the next items of this CTA, a bit each: whether there are rows
+    int known = 0;
     for (int tile = PAIR && crank != 0 ? p.num_items : tile_first; ok && tile < p.num_items; tile += tile_stride) {
-      if (nothing_next) {
-        nothing_next = empty_item(tile + tile_stride);
-        continue;
+      if constexpr (SKIP) {
+        if (known == 0) {
+          to_do = __ballot_sync(0xffffffffu, lane * tile_stride < p.num_items - tile && w8_tile<PAIR>(p, tile + lane * tile_stride, crank).rows > 0);
+          known = 32;
+        }
+        const uint32_t none = ~to_do & 1u;
+        to_do >>= 1;
+        --known;
+        if (none) continue;
       }
-      // Whether the next item is empty is looked up behind a few k blocks' MMAs, which keep the tensor core busy meanwhile.
-      const int look_up = min(kb_begin + 2, kb_end - 1);
       const uint32_t bn = (uint32_t)((tile < p.split_from) ? p.bn : (p.bn >> 1));
       const uint32_t idesc = make_idesc(ACC_S32, FMT_S8, FMT_S8, 0, B_NK ? 0 : 1, PAIR ? 2 * W8_BM : W8_BM, bn);
       const int buf = it & 1;
@@ -372,7 +376,6 @@ w8a8_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           if constexpr (PAIR) umma_commit_pair(&empty[stage]);
           else umma_commit(&empty[stage]);
         }
-        if (SKIP && kb == look_up) nothing_next = empty_item(tile + tile_stride);
         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
       }
       if (ok && elect_one_sync()) {  // the elected lane is the same one every time
