@@ -355,6 +355,10 @@ int qgemm_act_quant(const void* X, int8_t* Y, float* S, int64_t M, int64_t N, in
  * logits: [T, E] F16 / BF16 / F32.  bias: nullable fp32 [E].  weights: [T, top_k] fp32.  experts: [T, top_k] int32.
  * E <= 1024, top_k <= 32, num_groups <= 32.
  */
+#define QGEMM_MOE_MAX_EXPERTS 1024
+#define QGEMM_MOE_MAX_TOP_K 32
+#define QGEMM_MOE_MAX_GROUPS 32
+#define QGEMM_MOE_MAX_BLOCK_M 128
 #define QGEMM_ROUTE_SOFTMAX 0
 #define QGEMM_ROUTE_SIGMOID 1
 int qgemm_moe_route(const void* logits, const float* bias, float* weights, int32_t* experts, int64_t T, int64_t E,

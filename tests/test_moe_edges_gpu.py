@@ -202,3 +202,26 @@ def test_grouped_product_of_many_entries_per_cta(K, N, layout):
         assert len(table) * ((N + 255) // 256) > 32 * 148
         got = q.grouped_quant_matmul(A, B, table.cuda(), s, sa, out_dtype=BF16, b_layout=layout)
         assert torch.equal(got, want)
+
+
+# --------------------------------------------------------------------------------------------------------- limits of the counts
+def test_counts_beyond_the_limits_are_refused_before_anything_is_allocated():
+    l, e = torch.zeros((4, 64), device="cuda"), torch.zeros((4, 2), dtype=torch.int32, device="cuda")
+    torch.cuda.synchronize()
+    held = torch.cuda.memory_reserved()
+    for n in (1025, 10 ** 10, 10 ** 12, 2 ** 63, 2 ** 64 + 5, 10 ** 30):
+        with pytest.raises(q.QGemmError):
+            q.moe_block_metadata(e, n)
+        with pytest.raises(q.QGemmError):
+            q.moe_block_metadata(e, 4, block_M=n)
+        with pytest.raises(q.QGemmError):
+            q.moe_route(l, n)
+        for name in ("num_groups", "top_groups", "group_top"):
+            with pytest.raises(q.QGemmError):
+                q.moe_route(l, 2, **{name: n})
+        for kw in (dict(top_k=n), dict(top_k=2, num_groups=n), dict(top_k=2, group_top=2 ** 32 + 2)):
+            with pytest.raises(q.QGemmError):
+                q.moe_route(l, **kw, stream=torch.cuda.current_stream())
+        with pytest.raises(q.QGemmError):
+            q.moe_block_metadata(e, n, stream=torch.cuda.current_stream())
+    assert torch.cuda.memory_reserved() <= held + (4 << 20)

@@ -437,7 +437,7 @@ PyObject* h_moe_route(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (b == nullptr || b->dim() != 1 || b->size(0) != E || !same_device(*l, b)) Py_RETURN_NONE;
   }
   const int64_t k = as_int(args[1]), scoring = as_int(args[3]), groups = as_int(args[4]), top_groups = as_int(args[5]), group_top = as_int(args[6]);
-  if (T == 0 || k <= 0 || k > E || scoring < 0 || groups <= 0 || top_groups <= 0 || group_top < 1 || group_top > 2) Py_RETURN_NONE;
+  if (T == 0 || k <= 0 || k > E || k > QGEMM_MOE_MAX_TOP_K || scoring < 0 || groups <= 0 || top_groups <= 0 || group_top < 1 || group_top > 2) Py_RETURN_NONE;
   if (args[7] != Py_True && args[7] != Py_False) Py_RETURN_NONE;
   int64_t whole = 0;
   if (!PyFloat_CheckExact(args[8]) && !plain_int(args[8], &whole)) Py_RETURN_NONE;
@@ -465,10 +465,12 @@ PyObject* h_moe_blocks(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const at::Tensor* x = plain(args[0], at::kInt);
   if (x == nullptr || x->dim() != 2 || x->numel() == 0) Py_RETURN_NONE;
   const int64_t E = as_int(args[1]), bm = as_int(args[2]), R = x->numel();
-  if (E <= 0 || bm <= 0) Py_RETURN_NONE;
+  if (E <= 0 || E > QGEMM_MOE_MAX_EXPERTS || bm <= 0) Py_RETURN_NONE;
+  const int64_t blocks = api.moe_block_count(R, E, bm);
+  if (blocks > QGEMM_MOE_MAX_BLOCKS) Py_RETURN_NONE;
   const int dev = x->get_device();
   c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
-  at::Tensor meta = empty_cuda({api.moe_block_count(R, E, bm), 3}, at::kInt, dev), rows = empty_cuda(x->sizes(), at::kInt, dev),
+  at::Tensor meta = empty_cuda({blocks, 3}, at::kInt, dev), rows = empty_cuda(x->sizes(), at::kInt, dev),
              sizes = empty_cuda({E}, at::kInt, dev);
   void* st = c10::cuda::getCurrentCUDAStream((c10::DeviceIndex)dev).stream();
   int rc;

@@ -19,6 +19,9 @@ using namespace qgh;
 bool aligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 constexpr int kMaxDevices = 64;
+static_assert(QGEMM_MOE_MAX_EXPERTS == qg::RT_MAX_E && QGEMM_MOE_MAX_EXPERTS == qg::MB_MAX_E && QGEMM_MOE_MAX_TOP_K == qg::RT_MAX_K &&
+                  QGEMM_MOE_MAX_GROUPS == qg::RT_MAX_GROUPS,
+              "the limits that the header states are the kernels'");
 
 // A persistent kernel: as many blocks as the SMs hold, or as many as there are rows for.  `resident`: blocks per SM by device, once asked.
 template <typename P>
@@ -106,14 +109,14 @@ int qgemm_moe_route(const void* logits, const float* bias, float* weights, int32
                     int64_t num_groups, int64_t top_groups, int group_top, int scoring, int renormalize, float scale, int logits_dtype,
                     void* stream) {
   if (T < 0 || T > (1ll << 30)) return fail("qgemm_moe_route: 0 to 2^30 tokens (got %lld)", (long long)T);
-  if (E < 1 || E > qg::RT_MAX_E) return fail("qgemm_moe_route: 1 to %d experts (got %lld)", qg::RT_MAX_E, (long long)E);
-  if (num_groups < 1 || num_groups > qg::RT_MAX_GROUPS || E % num_groups != 0)
+  if (E < 1 || E > QGEMM_MOE_MAX_EXPERTS) return fail("qgemm_moe_route: 1 to %d experts (got %lld)", QGEMM_MOE_MAX_EXPERTS, (long long)E);
+  if (num_groups < 1 || num_groups > QGEMM_MOE_MAX_GROUPS || E % num_groups != 0)
     return fail("qgemm_moe_route: num_groups must be 1 to %d and divide the number of experts (got %lld groups, %lld experts)",
-                qg::RT_MAX_GROUPS, (long long)num_groups, (long long)E);
+                QGEMM_MOE_MAX_GROUPS, (long long)num_groups, (long long)E);
   if (top_groups < 1 || top_groups > num_groups)
     return fail("qgemm_moe_route: top_groups must be 1 to num_groups (got %lld of %lld)", (long long)top_groups, (long long)num_groups);
-  if (top_k < 1 || top_k > qg::RT_MAX_K || top_k > E / num_groups * top_groups)
-    return fail("qgemm_moe_route: top_k must be 1 to %d and no more than the %lld experts of top_groups groups (got %lld)", qg::RT_MAX_K,
+  if (top_k < 1 || top_k > QGEMM_MOE_MAX_TOP_K || top_k > E / num_groups * top_groups)
+    return fail("qgemm_moe_route: top_k must be 1 to %d and no more than the %lld experts of top_groups groups (got %lld)", QGEMM_MOE_MAX_TOP_K,
                 (long long)(E / num_groups * top_groups), (long long)top_k);
   if (group_top != 1 && group_top != 2) return fail("qgemm_moe_route: group_top must be 1 or 2 (got %d)", group_top);
   if (scoring != QGEMM_ROUTE_SOFTMAX && scoring != QGEMM_ROUTE_SIGMOID) return fail("qgemm_moe_route: unknown scoring %d", scoring);
@@ -154,8 +157,9 @@ int64_t qgemm_moe_block_count(int64_t entries, int64_t num_experts, int64_t bloc
 int qgemm_moe_blocks(const int32_t* experts, int32_t* block_metadata, int32_t* rows, int32_t* sizes, int64_t entries, int64_t num_experts,
                      int64_t block_M, void* stream) {
   if (entries < 0 || entries > (1ll << 30)) return fail("qgemm_moe_blocks: 0 to 2^30 entries (got %lld)", (long long)entries);
-  if (num_experts < 1 || num_experts > qg::MB_MAX_E) return fail("qgemm_moe_blocks: 1 to %d experts (got %lld)", qg::MB_MAX_E, (long long)num_experts);
-  if (block_M < 1 || block_M > 128) return fail("qgemm_moe_blocks: block_M must be 1 to 128 (got %lld)", (long long)block_M);
+  if (num_experts < 1 || num_experts > QGEMM_MOE_MAX_EXPERTS) return fail("qgemm_moe_blocks: 1 to %d experts (got %lld)", QGEMM_MOE_MAX_EXPERTS, (long long)num_experts);
+  if (block_M < 1 || block_M > QGEMM_MOE_MAX_BLOCK_M)
+    return fail("qgemm_moe_blocks: block_M must be 1 to %d (got %lld)", QGEMM_MOE_MAX_BLOCK_M, (long long)block_M);
   if (qgemm_moe_block_count(entries, num_experts, block_M) > QGEMM_MOE_MAX_BLOCKS)
     return fail("qgemm_moe_blocks: no more than %d blocks (got %lld entries in blocks of %lld)", QGEMM_MOE_MAX_BLOCKS, (long long)entries, (long long)block_M);
   if (sizes == nullptr || (entries > 0 && (experts == nullptr || block_metadata == nullptr || rows == nullptr)))

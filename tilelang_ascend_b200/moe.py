@@ -23,6 +23,9 @@ from .ops import _check_tensor, _ptr, _require_cuda, _stream_handle
 _ROUTE_DT = {torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16, torch.float32: _lib.DT_F32}
 _HALF_DT = {torch.float16: _lib.DT_F16, torch.bfloat16: _lib.DT_BF16}
 _SCORING = {"softmax": 0, "sigmoid": 1}
+# The limits of include/qgemm.h.  Counts above them are refused before outputs of that size are allocated.
+_MOST = {"top_k": 32, "num_experts": 1024, "block_M": 128, "num_groups": 32, "top_groups": 32, "group_top": 2}
+_MAX_BLOCKS = 715827882
 
 
 def _check_2d(t, idx, name, dtypes, device=None):
@@ -38,6 +41,8 @@ def _check_counts(**counts):
     for name, v in counts.items():
         if not isinstance(v, int) or v < 1:
             raise ValueError(f"{name} must be a positive integer, got {v!r}")
+        if v > _MOST[name]:
+            raise _lib.QGemmError(f"{name} must be 1 to {_MOST[name]}, got {v}")
 
 
 def moe_route(logits, top_k, bias=None, scoring="softmax", num_groups=1, top_groups=1, group_top=2, renormalize=True, scale=1.0,
@@ -91,7 +96,10 @@ def moe_block_metadata(experts, num_experts, block_M=128, stream=None):
     dev = experts.device
     _check_counts(num_experts=num_experts, block_M=block_M)
     E, bm, R = num_experts, block_M, experts.numel()
-    meta = torch.empty((lib.qgemm_moe_block_count(R, E, bm), 3), dtype=torch.int32, device=dev)
+    blocks = lib.qgemm_moe_block_count(R, E, bm)
+    if blocks > _MAX_BLOCKS:
+        raise _lib.QGemmError(f"no more than {_MAX_BLOCKS} blocks, got {R} picks in blocks of {bm}")
+    meta = torch.empty((blocks, 3), dtype=torch.int32, device=dev)
     rows = torch.empty(experts.shape, dtype=torch.int32, device=dev)
     sizes = torch.empty((E,), dtype=torch.int32, device=dev)
     with torch.cuda.device(dev):
