@@ -8,7 +8,8 @@
 // The picks are those of the real numbers: two scores that fp32 cannot tell apart must not depend on how a kernel adds.  Without
 // a bias the logits themselves are compared (both score functions are increasing).  With one, or with sums of two scores, fp32
 // values are compared and a token whose decision is nearer than the error of the fp32 scores is decided again in fp64 (random
-// scores: one token in some hundreds).
+// scores: one token in some hundreds; what fp64 gives the same number is a tie).  That error goes by the largest finite bias: one of -1e9 among
+// others of 0.1 sends every token there, 16384 x 256 with groups 75 us instead of 25 (-inf, which takes an expert out, 26).
 //
 // One warp per token.  The experts of a group are dealt to a power of two of lanes, so that shuffles settle it whatever its size
 // (through shared memory 8000 x 160 in 8 groups was 17.3 us instead of 10.9).  A lane has up to V consecutive experts as 32-bit keys
@@ -21,11 +22,12 @@
 #pragma once
 
 #include "common.cuh"
+#include "packed_float.cuh"
 
 namespace qg {
 
 constexpr int RT_WARPS = 4;       // warps of a block, a token each
-constexpr int RT_MAX_E = 1024;    // experts: 32 per lane
+constexpr int RT_MAX_E = 1024;    // experts: 32 per lane, up to 60 where groups leave lanes idle
 constexpr int RT_MAX_K = 32;      // picks: one per lane
 constexpr int RT_MAX_GROUPS = 32; // groups: one per lane
 
@@ -61,16 +63,10 @@ __device__ __forceinline__ bool rt_equal(const MoeRouteParams& p, const void* ro
   return rt_load<DT>(row, e) == rt_load<DT>(row, f) && (by_logits || ld_written(p.bias + e) == ld_written(p.bias + f));
 }
 
-// The larger value, or NaN if either is one.
-__device__ __forceinline__ float rt_max(float a, float b) {
-  float v;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(a), "f"(b));
-  return v;
-}
-
 // Values as unsigned numbers of the same order; NaN above everything, both zeros alike, -inf (not offered) at RT_NONE.
 constexpr int RT_LIST = 72;  // two lists of 36 entries of a warp, on a 16-byte boundary
-__host__ __device__ constexpr int rt_smem_bytes(int E) { return 8 * (RT_WARPS * E + (RT_WARPS * E & 1) + RT_WARPS * RT_LIST); }
+__host__ __device__ constexpr int rt_smem_bytes(int E) { return 8 * (RT_WARPS * E + RT_WARPS * RT_LIST); }
+static_assert(RT_WARPS % 2 == 0, "the lists, behind the warps' keys, start on a 16-byte boundary");
 
 template <typename K> struct RtKey;
 template <> struct RtKey<uint32_t> {
@@ -225,22 +221,12 @@ __device__ __noinline__ int rt_rank_in_64(const MoeRouteParams& p, const void* r
   return lane < n ? rank : lane;
 }
 
-__device__ __forceinline__ float rt_exp2(float t) {
-  float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-  return e;
-}
-__device__ __forceinline__ float rt_rcp(float d) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
-  return r;
-}
 constexpr float RT_LOG2E = 1.4426950408889634f;
 // Off by less than 2^-21: the error of exp, 2^-22 + |l| 7.5e-8, enters times s (1 - s), and sum and reciprocal add 1.5 * 2^-23.
-__device__ __forceinline__ float rt_sigmoid(float l) { return rt_rcp(1.0f + rt_exp2(-RT_LOG2E * l)); }
+__device__ __forceinline__ float rt_sigmoid(float l) { return rcp_approx(1.0f + ex2_approx(-RT_LOG2E * l)); }
 // exp(l - top) to 2^-22 + |l - top| 7.5e-8, relative: the argument's rounding is put right behind the approximation.
 __device__ __forceinline__ float rt_exp_below(float l, float top) {
-  const float x = l - top, t = x * RT_LOG2E, e = rt_exp2(t);
+  const float x = l - top, t = x * RT_LOG2E, e = ex2_approx(t);
   return x < -100.0f ? 0.0f : fmaf(e, fmaf(x, RT_LOG2E, -t) * 0.6931471806f, e);
 }
 
@@ -331,7 +317,7 @@ __global__ void __launch_bounds__(RT_WARPS * 32, rt_min_blocks(V)) moe_route_ker
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   unsigned long long* keys64 = rt_smem + (size_t)warp * p.E;
   // candidates, and what is in each place of the order: (expert backwards, value)
-  uint2* list = reinterpret_cast<uint2*>(rt_smem + (size_t)RT_WARPS * p.E + (RT_WARPS * p.E & 1)) + warp * RT_LIST;
+  uint2* list = reinterpret_cast<uint2*>(rt_smem + (size_t)RT_WARPS * p.E) + warp * RT_LIST;
   uint2* place = list + RT_LIST / 2;
   // Lanes of a power of two to a group, so that it is settled by shuffles; in the order of the experts.
   const int share = 1 << p.log_share, part = lane & (share - 1), my_group = lane >> p.log_share;
@@ -414,8 +400,10 @@ __global__ void __launch_bounds__(RT_WARPS * 32, rt_min_blocks(V)) moe_route_ker
     }
 #pragma unroll
     for (int i = 0; i < V; ++i) key[i / L][i % L] = (K::of(c[i]) & ~PLACE) | (PLACE - i);
-    // How near two c may come before fp32 cannot tell them apart: each is off by 2^-21 of the largest score that there can be, by its
-    // rounding and by the bits of the place.
+    // How near two c may come before fp32 cannot tell them apart, in units of 2^-24 of the largest score that there can be.  sigmoid: 8 each
+    // (rt_sigmoid), 16.  softmax: the exponentials 4 each (what smaller ones are off by is less), their products with 1 / sum 1 each, and
+    // the sum, whose V + 4 additions, exponentials and division move all scores alike, V + 9: V + 19.  Then, of the largest score
+    // and bias, the sum with the bias 1 each and the bits that the place takes 2 (V - 1) of either.  3 V + 19 in all, of the 20 + 4 V here.
     const float score = p.softmax && !by_logits ? inv_sum : 1.0f;
     const float tol = 0x1p-20f * score + (0x1p-22f + V * 0x1p-22f) * (most_bias + score);
     bool near = false, kept = true;

@@ -1,9 +1,22 @@
-// Two fp32 values in a 64-bit register: sm_100a's packed instructions do in one issue what two would, with the same rounding.
+// fp32 arithmetic of the operators that are bound by issue: approximate exp2 and reciprocal, and two values in a 64-bit register,
+// for which sm_100a's packed instructions do in one issue what two would, with the same rounding.
 #pragma once
 
 #include "common.cuh"
 
 namespace qg {
+
+// 2^t to 2^-22, 1 / d to 2^-23; subnormal results are 0.
+__device__ __forceinline__ float ex2_approx(float t) {
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  return e;
+}
+__device__ __forceinline__ float rcp_approx(float d) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+  return r;
+}
 
 using f32x2 = unsigned long long;
 __device__ __forceinline__ f32x2 f2_make(float lo, float hi) {

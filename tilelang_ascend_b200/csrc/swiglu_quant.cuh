@@ -37,22 +37,12 @@ struct SwigluQuantParams {
 };
 
 // --------------------------------------------------------------------------------------------------- a in fp32 and fp64
-__device__ __forceinline__ float sq_exp2(float t) {
-  float e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
-  return e;
-}
-__device__ __forceinline__ float sq_rcp(float d) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
-  return r;
-}
 __device__ __forceinline__ f32x2 sq_gate(f32x2 g, f32x2 u) {
   const float L = -1.4426950408889634f;  // -log2(e)
   float t0, t1, d0, d1;
   f2_get(f2_mul(g, f2_make(L, L)), t0, t1);
-  f2_get(f2_add(f2_make(sq_exp2(t0), sq_exp2(t1)), f2_make(1.0f, 1.0f)), d0, d1);
-  return f2_mul(f2_mul(g, f2_make(sq_rcp(d0), sq_rcp(d1))), u);
+  f2_get(f2_add(f2_make(ex2_approx(t0), ex2_approx(t1)), f2_make(1.0f, 1.0f)), d0, d1);
+  return f2_mul(f2_mul(g, f2_make(rcp_approx(d0), rcp_approx(d1))), u);
 }
 template <bool BF16>
 __device__ __forceinline__ float sq_float(uint32_t bits) {
@@ -304,7 +294,7 @@ __global__ void __launch_bounds__(sq_block(TPR), sq_min_blocks(TPR, KEEP)) swigl
     if (p.round_scale) scale = aq_pow2_ceil(scale);
     if (!finite) scale = __uint_as_float(m);  // inf or NaN: it stays one
     if (t == 0) p.S[row] = scale;
-    const float rcp = sq_rcp(scale);
+    const float rcp = rcp_approx(scale);
     const float share = finite ? rcp * (off + 2.5e-7f) : 0.0f;  // what a quotient may be off by, per |a|
     uint2* y = reinterpret_cast<uint2*>(p.Y) + (long long)row * chunks;
     const f32x2 rcp2 = f2_make(rcp, rcp);
