@@ -350,8 +350,10 @@ int qgemm_act_quant(const void* X, int8_t* Y, float* S, int64_t M, int64_t N, in
  *   experts    = the top_k largest c offered in groups that stay, in that order (ties: the lower index), -1 where
  *                there are no more
  *   weights[j] = s[experts[j]], with `renormalize` divided by their sum, times `scale`; 0 where there is no expert
- * The picks are those of the exact scores (without a bias the logits are compared; with one, decisions that are nearer
- * than the error of fp32 are taken in fp64).  A NaN logit counts as largest and makes its token's weights NaN.
+ * The picks are those of the exact scores (without a bias the logits are compared; with one, and for sums of two scores, decisions that are
+ * nearer than the error of fp32 are taken in fp64, and what fp64 gives the same number is a tie).  A NaN logit counts as largest; its
+ * weight is NaN, and with softmax or `renormalize` so are all of its token's.  An expert is taken out by -inf; a finite bias far
+ * below the others does so too, but makes every decision a near one (some three times slower).
  * logits: [T, E] F16 / BF16 / F32.  bias: nullable fp32 [E].  weights: [T, top_k] fp32.  experts: [T, top_k] int32.
  * E <= 1024, top_k <= 32, num_groups <= 32.
  */

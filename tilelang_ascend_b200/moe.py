@@ -55,7 +55,8 @@ def moe_route(logits, top_k, bias=None, scoring="softmax", num_groups=1, top_gro
     largest ``s + bias``.  The weights are the chosen ``s``, divided by their sum if ``renormalize``, times ``scale``.
 
     An expert whose logit (or bias) is -inf is never chosen; where a token has fewer than ``top_k`` left, its last experts are
-    -1 with weight 0 (a padding token: a row of -inf).  A NaN logit counts as largest and makes its token's weights NaN."""
+    -1 with weight 0 (a padding token: a row of -inf).  Mask by -inf: a finite bias far below the others gives the same picks, but more
+    slowly.  A NaN logit counts as largest; its weight is NaN, and with softmax or ``renormalize`` so are all of its token's."""
     if stream is None and scoring in _SCORING:
         we = (ops._host or ops._native()).moe_route(logits, top_k, bias, _SCORING[scoring], num_groups, top_groups, group_top, renormalize, scale)
         if we is not None:
