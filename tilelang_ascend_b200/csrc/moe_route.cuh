@@ -17,8 +17,8 @@
 // value that top_k lanes' heads reach bounds the picks from below: a maximum over the heads, one redux instruction, top_k times.  The
 // keys from there on, a dozen or so, are gathered by votes and each lane counts how many come before its own.  (A maximum over the
 // heads per pick, with a step of the winner's list, was 32 instructions a pick; this is 130 for all.)  What bounds it is issue:
-// 16384 x 256 in bf16 with bias and groups is 1.5 us of memory and 815 instructions of a warp per token, 12 us at one a cycle;
-// measured 21.7.
+// 16384 x 256 in bf16 with bias and groups is 1.5 us of memory and 792 instructions of a warp per token, 11 us at one a cycle;
+// measured 21.6.
 #pragma once
 
 #include "common.cuh"
