@@ -230,14 +230,6 @@ __device__ __forceinline__ float rt_exp_below(float l, float top) {
   return x < -100.0f ? 0.0f : fmaf(e, fmaf(x, RT_LOG2E, -t) * 0.6931471806f, e);
 }
 
-// sigmoid of every lane's logit times exp(-the largest of them), where that is negative: what fp32 does not hold otherwise.
-__device__ __noinline__ float rt_small_scores(float l, bool there) {
-  using K = RtKey<uint32_t>;
-  const float most = fminf(K::value(K::warp_max(K::of(l))), 0.0f);
-  const float s = l >= 0.0f ? __fdividef(1.0f, 1.0f + expf(-l)) : __fdividef(expf(l - most), 1.0f + expf(l));
-  return there ? s : 0.0f;
-}
-
 // Largest first.
 template <int L>
 __device__ __forceinline__ void rt_sort(uint32_t (&k)[L]) {
@@ -583,14 +575,15 @@ __global__ void __launch_bounds__(RT_WARPS * 32, rt_min_blocks(V)) moe_route_ker
     // exact where all the picked scores are tiny.
     float s;
     if (p.renormalize) {
-      if (p.softmax) {
+      if (p.softmax || __all_sync(0xffffffffu, lp < -30.0f)) {
         const float most = K::value(K::warp_max(K::of(lp)));  // a NaN among the picks is on top
         s = there ? expf(lp - most) : 0.0f;
         if (need_top) s += top - top;  // the sum of all scores is NaN where a logit is NaN or +inf
-      } else if (__any_sync(0xffffffffu, there && lp < -30.0f)) {
-        s = rt_small_scores(lp, there);
       } else {
-        s = there ? __fdividef(1.0f, 1.0f + expf(-lp)) : 0.0f;
+        // times 2^46, so that scores below fp32's range, as exp(l) in two factors, are in it
+        const float e = expf(lp < -30.0f ? 0.5f * lp : -lp);
+        s = lp < -30.0f ? e * (e * 0x1p46f) : __fdividef(0x1p46f, 1.0f + e);
+        if (!there) s = 0.0f;
       }
       float all = s;
 #pragma unroll
